@@ -48,6 +48,10 @@ class StatusReport(C.Structure):
                 ("seq", C.c_uint64)]
 
 
+class GradTensor(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("len_elements", C.c_size_t), ("dtype_in", C.c_int), ("dtype_out", C.c_int)]
+
+
 _lib = None
 _fast = None
 
@@ -100,6 +104,13 @@ def _declare(lib) -> None:
         "ibcomm_emu_set_direct_staging": [vp, i],
         "ibcomm_emu_last_status": [vp, C.POINTER(StatusReport)],
         "ibcomm_copy_scale": [vp, vp, sz, i, i, dbl, vp],
+        "ibcomm_grad_norm": [C.POINTER(GradTensor), i, i, vp, i, vp, vp, i, vp, vp],
+        "ibcomm_clip_grads": [C.POINTER(GradTensor), i, i, dbl, vp, i, vp, vp, i, vp],
+        "ibcomm_grad_sum_host": [C.POINTER(GradTensor), i, i, C.POINTER(dbl)],
+        "ibcomm_scale_grads_host": [C.POINTER(GradTensor), i, dbl],
+        "ibcomm_embedding": [vp, i, sz, vp, i, sz, sz, vp, i, dbl, vp],
+        "ibcomm_embedding_grad_work": [sz, sz, sz, C.POINTER(sz)],
+        "ibcomm_embedding_grad": [vp, i, sz, vp, i, vp, i, sz, sz, C.c_int64, dbl, i, vp, sz, vp],
         "ibcomm_parse_number": [C.c_char_p, C.POINTER(C.c_int64)],
         "ibcomm_get_exp_of_two": [C.c_uint64],
         "ibcomm_set_tunable": [C.c_char_p, i],

@@ -62,6 +62,8 @@ CUDA_SOURCES = [
     "src/cuda/hybrid_kernel.cu",
     "src/cuda/staged_kernel.cu",
     "src/cuda/copy_kernel.cu",
+    "src/cuda/grad_norm_kernel.cu",
+    "src/cuda/embedding_kernel.cu",
     "src/cuda/p2p_sendrecv.cu",
     "src/cuda/no_alloc.cu",
 ]

@@ -1,0 +1,104 @@
+"""Embedding lookup with scaling, and the gradient of its table.
+
+The gradient is summed by sorted tokens: every row of the table is written once, by one warp per slice of its columns,
+in float32 and in the order of the tokens.  It is the same for the same inputs, whatever ran beside it, so ranks that
+hold replicas agree; and it can be added straight into a gradient bucket, where only the rows that tokens name are
+touched.  Tokens outside of the table give a row of zeros and no gradient: padded places (-1), or the tokens of another
+rank's part of a table that is split by rows (look up ``tokens - first_row`` and allreduce the rows)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+from .._native import IbcommError
+from ..parallel.communicator import dtype_code
+
+
+def _check(tokens: torch.Tensor, padding_idx: Optional[int], rows: int) -> int:
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise IbcommError(_native.NOT_SUPPORTED, f"tokens are int32 or int64, got {tokens.dtype}")
+    if padding_idx is None:
+        return -1
+    if not 0 <= padding_idx < rows:
+        raise IbcommError(_native.INVALID_ARGUMENT, f"padding_idx {padding_idx} is no row of {rows}")
+    return int(padding_idx)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, padding, out_code, grad_into):
+        ctx.save_for_backward(tokens)
+        ctx.weight = weight
+        ctx.scale, ctx.padding, ctx.grad_into = scale, padding, grad_into
+        return _native.fast().embedding(tokens, weight, out_code, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (tokens,) = ctx.saved_tensors
+        into, weight = ctx.grad_into, ctx.weight
+        if into is None:
+            into = torch.empty(weight.shape, dtype=weight.dtype, device=grad.device)
+            _native.fast().embedding_grad(tokens, grad.contiguous(), into, ctx.padding, ctx.scale, False)
+            return into, None, None, None, None, None
+        _native.fast().embedding_grad(tokens, grad.contiguous(), into, ctx.padding, ctx.scale, True)
+        if weight.is_leaf and weight.grad is not None:
+            # A gradient without entries costs nothing to add, and takes the way of every other one: autograd makes the
+            # stream of `weight.grad` wait for this one, adds other uses of the table and runs the bucket's hook, in that order.
+            none = torch.sparse_coo_tensor(size=weight.shape, dtype=weight.dtype, device=weight.device, check_invariants=False)
+            return none, None, None, None, None, None
+        # Where nothing is handed on, the stream of the backward call waits at its end.
+        done = torch.cuda.current_stream(into.device).record_event()
+        torch.autograd.Variable._execution_engine.queue_callback(
+            lambda: torch.cuda.current_stream(into.device).wait_event(done))
+        return None, None, None, None, None, None
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
+              out_dtype=None, grad_into: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``scale * weight[tokens]``, of shape ``tokens.shape + (width,)`` and type ``out_dtype`` (default: the table's).
+
+    ``tokens`` int32 or int64, ``weight`` ``(rows, width)`` float32, float16 or bfloat16; on the current stream.
+    Differentiable in ``weight``: its gradient is summed in float32 and comes in the table's type, without the row
+    ``padding_idx``.  With ``grad_into`` (a tensor of the table's shape, such as its view in a gradient bucket) the
+    backward pass adds the gradient there instead, and autograd has nothing to add to ``weight.grad``."""
+    padding = _check(tokens, padding_idx, weight.shape[0] if weight.dim() == 2 else 0)
+    out_code = -1 if out_dtype is None else dtype_code(out_dtype)
+    tokens = tokens.contiguous()
+    if grad_into is not None:
+        if grad_into.shape != weight.shape or not grad_into.is_contiguous() or grad_into.device != weight.device:
+            raise IbcommError(_native.INVALID_ARGUMENT, "grad_into must be contiguous, of the table's shape and on its GPU")
+        if grad_into.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise IbcommError(_native.NOT_SUPPORTED, f"no embedding of {grad_into.dtype}")
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(weight, tokens, float(scale), padding, out_code, grad_into)
+    return _native.fast().embedding(tokens, weight, out_code, float(scale))
+
+
+def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+                   num_rows: Optional[int] = None, dtype=None, accumulate: bool = False, scale: float = 1.0,
+                   padding_idx: Optional[int] = None) -> torch.Tensor:
+    """The gradient of :func:`embedding`'s table: row ``v`` = ``scale`` times the sum of ``grad``'s rows at the places
+    where ``tokens`` is ``v``.
+
+    ``out`` (contiguous, ``(rows, width)``) is overwritten, rows without tokens with zeros; with ``accumulate`` the sums
+    are added to it and only rows that tokens name are touched.  Without ``out`` a table of ``num_rows`` rows in ``dtype``
+    (default: ``grad``'s) is made.  Types float32, float16, bfloat16 in any mixture; sums in float32, rounded once.
+    ``tokens`` and ``grad`` may come from several ranks (``all_gather`` both): with many rows that few tokens name, that is
+    less to send than the table's gradient."""
+    if out is None:
+        if num_rows is None or num_rows < 0 or accumulate:
+            raise IbcommError(_native.INVALID_ARGUMENT, "give out, or num_rows without accumulate")
+        if grad.dim() < 1:
+            raise IbcommError(_native.INVALID_ARGUMENT, "grad must hold a row of the table's width for every token")
+        padding = _check(tokens, padding_idx, num_rows)
+        out = torch.empty(num_rows, grad.shape[-1], dtype=dtype or grad.dtype, device=grad.device)
+    else:
+        if num_rows is not None or dtype is not None:
+            raise IbcommError(_native.INVALID_ARGUMENT, "out has its own rows and type")
+        padding = _check(tokens, padding_idx, out.shape[0] if out.dim() == 2 else 0)
+    _native.fast().embedding_grad(tokens.contiguous(), grad.contiguous(), out, padding, float(scale), bool(accumulate))
+    return out

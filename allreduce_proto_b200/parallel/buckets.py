@@ -150,6 +150,33 @@ class GradientBuckets:
         for buf, shard in zip(self.flat, mine):
             self.comm.all_gather(shard, buf, algo=algo, sync=sync)
 
+    # ----------------------------------------------------- norm and clipping
+    def grad_norm(self, *, norm_type: float = 2.0, sharded: bool = False) -> torch.Tensor:
+        """The norm of all gradients (call it after :meth:`allreduce` or :meth:`finish`).
+
+        ``sharded``: after :meth:`reduce_scatter`, from this rank's blocks and one value of every other rank's."""
+        from ..ops.gradients import grad_norm
+        return grad_norm(self.shards() if sharded else self.flat, norm_type=norm_type, comm=self.comm if sharded else None)
+
+    def clip_grad_norm(self, max_norm: float, *, norm_type: float = 2.0, sharded: bool = False) -> torch.Tensor:
+        """Scales the gradients (``sharded``: this rank's blocks) so that their norm is at most ``max_norm``, in
+        place, and returns the norm they had; see :func:`allreduce_proto_b200.ops.clip_grad_norm`."""
+        from ..ops.gradients import clip_grad_norm
+        return clip_grad_norm(self.shards() if sharded else self.flat, max_norm, norm_type=norm_type,
+                              comm=self.comm if sharded else None)
+
+    # ------------------------------------------------------------- embedding
+    def embedding(self, index: int, tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
+                  padding_idx: Optional[int] = None, out_dtype=None) -> torch.Tensor:
+        """``scale * weight[tokens]`` whose backward pass adds the table's gradient straight into ``views[index]``.
+
+        autograd would zero and fill a tensor of the table's size and add it to the bucket; here only the rows that
+        tokens name are read and written.  ``weight`` is the parameter that :meth:`attach` or
+        :meth:`overlap_with_backward` was given in that place; its hook runs as for every other gradient, and the same
+        table may have other uses in the step (a tied output layer)."""
+        from ..ops.embedding import embedding
+        return embedding(tokens, weight, scale=scale, padding_idx=padding_idx, out_dtype=out_dtype, grad_into=self.views[index])
+
     # ------------------------------------------------ overlap with backward
     def overlap_with_backward(self, params: Iterable[torch.nn.Parameter], *, average: bool = True, wire=None,
                               algo: str = "auto") -> None:

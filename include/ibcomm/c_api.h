@@ -141,6 +141,42 @@ int ibcomm_emu_last_status(ibcomm_emu* w, ibcomm_status_report* out);
 /* out[i] = cast(in[i] * scale) on the current device. */
 int ibcomm_copy_scale(const void* in, void* out, size_t len_elements, int dtype_in, int dtype_out, double scale, void* stream);
 
+/* ---- gradients: the norm of a list of tensors, clipping ----
+ * dtypes float32, float64, float16, bfloat16.  power: 2 = root of the sum of squares, 0 = largest magnitude (a NaN
+ * anywhere makes either NaN).  `out` = cast(in * min(1, max_norm / (norm + 1e-6))) where clipping: float32 to float32,
+ * float16, bfloat16; the 16-bit types to themselves and to float32; float64 to itself.  An `out` is its own `in`
+ * (in place) or shares no memory with any other tensor of the call. */
+typedef struct {
+  const void* in;
+  void* out; /* null for the norm alone */
+  size_t len_elements;
+  int dtype_in;
+  int dtype_out;
+} ibcomm_grad_tensor;
+/* On the current device, only enqueued.  `work`: IBCOMM_NORM_WORK doubles of device memory.  `norm` (float32, or float64
+ * with norm_dtype 1) and `sum` (the sum of squares or the maximum, float64) are device memory and may be null.  With
+ * `sums` not null its num_sums values, the ranks' sums, are joined instead of the tensors' own. */
+#define IBCOMM_NORM_WORK 2048
+int ibcomm_grad_norm(const ibcomm_grad_tensor* tensors, int count, int power, const double* sums, int num_sums, double* work,
+                     void* norm, int norm_dtype, double* sum, void* stream);
+int ibcomm_clip_grads(const ibcomm_grad_tensor* tensors, int count, int power, double max_norm, const double* sums, int num_sums,
+                      double* work, void* norm, int norm_dtype, void* stream);
+/* Host buffers (float32, float64): the sum of squares or the maximum, and cast(in * coefficient). */
+int ibcomm_grad_sum_host(const ibcomm_grad_tensor* tensors, int count, int power, double* sum);
+int ibcomm_scale_grads_host(const ibcomm_grad_tensor* tensors, int count, double coefficient);
+
+/* ---- embedding, on the current device, only enqueued; float32, float16, bfloat16 in any combination ----
+ * tokens: int32 (dtype 2) or int64 (3); those outside [0, rows) name no row.
+ * out[t] = cast(scale * weight[tokens[t]]), zeros where there is no row. */
+int ibcomm_embedding(const void* tokens, int tokens_dtype, size_t num_tokens, const void* weight, int weight_dtype, size_t rows,
+                     size_t width, void* out, int out_dtype, double scale, void* stream);
+/* out[v] = cast((accumulate ? out[v] : 0) + scale * sum of grad[t] over the t with tokens[t] == v, v != padding_row), summed in
+ * float32 in the order of t.  With accumulate only rows that tokens name are touched.  padding_row -1 = none. */
+int ibcomm_embedding_grad_work(size_t num_tokens, size_t rows, size_t width, size_t* bytes);
+int ibcomm_embedding_grad(const void* tokens, int tokens_dtype, size_t num_tokens, const void* grad, int grad_dtype, void* out,
+                          int out_dtype, size_t rows, size_t width, int64_t padding_row, double scale, int accumulate, void* work,
+                          size_t work_bytes, void* stream);
+
 /* Utilities. */
 int ibcomm_parse_number(const char* text, int64_t* out);
 

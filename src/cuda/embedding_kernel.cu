@@ -1,0 +1,513 @@
+// Embedding: out[t] = round(scale * weight[token[t]]), and the gradient of the
+// table: out[v] (+)= round(scale * sum of grad[t] over the tokens t that name v).
+//
+// The gradient sorts the tokens' positions by row (a stable radix sort, so that
+// the positions of a row stay in their order), cuts the sorted list into chunks
+// of kChunkTokens and gives every warp a chunk and a slice of the columns.  The
+// warp adds the rows of a run of equal tokens in fp32 registers; a run inside
+// the chunk is written at once, one that a chunk's edge cuts leaves partial sums
+// in the workspace, which a second kernel adds in the chunks' order.  No atomics
+// on values: the result does not depend on the order of execution.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "grad_ops.h"
+#include "ibcomm/communicator.h"
+#include "kernels.h"
+#include "vec_ops.cuh"
+
+namespace ibcomm {
+namespace dev {
+
+// kN values at `p` (aligned to their size, 16 bytes at most) as fp32, and back.
+template <typename T, int kN>
+__device__ __forceinline__ void LoadValues(const T* p, float* a) {
+  constexpr int kBytes = kN * static_cast<int>(sizeof(T));
+  if constexpr (kBytes >= 16) {
+#pragma unroll
+    for (int v = 0; v < kBytes / 16; ++v) VecIO<T>::Load(Ld16(p + v * VecIO<T>::kN), a + v * VecIO<T>::kN);
+  } else {
+    static_assert(kBytes == 8 && sizeof(T) == 2, "half a vector of 16-bit values");
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    float b[8];
+    VecIO<T>::Load(make_uint4(q.x, q.y, 0, 0), b);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) a[e] = b[e];
+  }
+}
+template <typename T, int kN>
+__device__ __forceinline__ void StoreValues(T* p, const float* a) {
+  constexpr int kBytes = kN * static_cast<int>(sizeof(T));
+  if constexpr (kBytes >= 16) {
+#pragma unroll
+    for (int v = 0; v < kBytes / 16; ++v) St16(p + v * VecIO<T>::kN, VecIO<T>::Store(a + v * VecIO<T>::kN));
+  } else {
+    static_assert(kBytes == 8 && sizeof(T) == 2, "half a vector of 16-bit values");
+    *reinterpret_cast<uint2*>(p) = make_uint2(VecIO<T>::P2(a[0], a[1]), VecIO<T>::P2(a[2], a[3]));
+  }
+}
+
+// ------------------------------------------------------------------ lookup
+constexpr int kLookupThreads = 256;
+
+template <typename TI, typename TO>
+struct LookupQuantum {
+  // 16 bytes of the narrower type at most: 16-bit values in eights, fp32 to fp32 in fours.
+  static constexpr int kN = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
+};
+
+template <bool kTokens64>
+__device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
+  if constexpr (kTokens64) return static_cast<const long long*>(tokens)[t];
+  else return static_cast<const int*>(tokens)[t];
+}
+
+// A thread per quantum of the output, kN values with kVector, else one.
+template <typename TI, typename TO, bool kTokens64, bool kVector>
+__global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
+                                                                  uint64_t quanta, uint32_t per_row, uint64_t rows, uint64_t width, float scale) {
+  constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1;
+  const uint64_t q = static_cast<uint64_t>(blockIdx.x) * kLookupThreads + threadIdx.x;
+  if (q >= quanta) return;
+  const uint64_t t = q / per_row;
+  const uint64_t column = (q - t * per_row) * kN;
+  const int64_t id = Token<kTokens64>(tokens, t);
+  const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
+  float a[kN];
+#pragma unroll
+  for (int e = 0; e < kN; ++e) a[e] = 0.f;
+  if (inside) {
+    const TI* p = weight + static_cast<uint64_t>(id) * width + column;
+    if constexpr (kVector) LoadValues<TI, kN>(p, a);
+    else a[0] = ToAcc<float, TI>(*p);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) a[e] *= scale;
+  }
+  TO* o = out + t * width + column;
+  if constexpr (kVector) StoreValues<TO, kN>(o, a);
+  else *o = FromAcc<TO, float>(a[0]);
+}
+
+// -------------------------------------------------------------------- sort
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kMostDigitBits = 10;
+constexpr int kMostSortBlocks = 64;
+
+struct SortParams {
+  const void* tokens;
+  int tokens_are_64;
+  uint32_t n;
+  uint32_t rows;       // also the key of tokens without a gradient
+  int64_t padding;
+  uint32_t per_block;  // a multiple of kSortThreads
+  int passes, bits;
+  uint32_t* key[2];
+  uint32_t* position[2];
+  uint32_t* counts;    // gridDim.x x bins
+};
+
+__device__ __forceinline__ uint32_t KeyOf(const SortParams& p, uint32_t t) {
+  const int64_t id = p.tokens_are_64 ? Token<true>(p.tokens, t) : Token<false>(p.tokens, t);
+  return id >= 0 && id < static_cast<int64_t>(p.rows) && id != p.padding ? static_cast<uint32_t>(id) : p.rows;
+}
+
+// A least-significant-digit radix sort, cooperative: a block's part of the list
+// is cut into one part per warp, a digit's count of every warp gives the places.
+// A warp places 32 elements at a time in their order, so every pass is stable.
+__global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
+  extern __shared__ uint32_t warp_counts[];  // kSortWarps x bins
+  __shared__ uint32_t scan[kSortWarps];
+  const cooperative_groups::grid_group grid = cooperative_groups::this_grid();
+  const int bins = 1 << p.bits;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t part = p.per_block / kSortWarps;
+  const uint32_t begin = blockIdx.x * p.per_block + warp * part;
+  const uint32_t end = min(begin + part, p.n);
+  uint32_t* mine = warp_counts + warp * bins;
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const uint32_t* key_in = p.key[(pass + 1) & 1];
+    const uint32_t* position_in = p.position[(pass + 1) & 1];
+    uint32_t* key_out = p.key[pass & 1];
+    uint32_t* position_out = p.position[pass & 1];
+    const int shift = pass * p.bits;
+    for (int i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads) warp_counts[i] = 0;
+    __syncthreads();
+    for (uint32_t i = begin + lane; i < end; i += 32) {
+      const uint32_t k = pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
+      atomicAdd(&mine[(k >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+      uint32_t sum = 0;
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = warp_counts[w * bins + d];
+        warp_counts[w * bins + d] = sum;
+        sum += c;
+      }
+      __stcg(p.counts + static_cast<size_t>(blockIdx.x) * bins + d, sum);
+    }
+    grid.sync();
+    // Places of this block's elements of digit d: behind all smaller digits and behind digit d of the blocks before.
+    uint32_t carried = 0;
+    for (int d0 = 0; d0 < bins; d0 += kSortThreads) {
+      const int d = d0 + threadIdx.x;
+      uint32_t total = 0, before = 0;
+      if (d < bins) {
+        for (uint32_t g = 0; g < gridDim.x; ++g) {
+          const uint32_t c = __ldcg(p.counts + static_cast<size_t>(g) * bins + d);
+          before += g < blockIdx.x ? c : 0;
+          total += c;
+        }
+      }
+      uint32_t inclusive = total;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inclusive, s);
+        if (lane >= s) inclusive += v;
+      }
+      if (lane == 31) scan[warp] = inclusive;
+      __syncthreads();
+      uint32_t base = carried, all = 0;
+      for (int w = 0; w < kSortWarps; ++w) {
+        base += w < warp ? scan[w] : 0;
+        all += scan[w];
+      }
+      carried += all;
+      if (d < bins) {
+        const uint32_t place = base + inclusive - total + before;
+        for (int w = 0; w < kSortWarps; ++w) warp_counts[w * bins + d] += place;
+      }
+      __syncthreads();
+    }
+    for (uint32_t i0 = begin; i0 < end; i0 += 32) {
+      const uint32_t i = i0 + lane;
+      const bool valid = i < end;
+      const unsigned active = __ballot_sync(0xffffffffu, valid);
+      if (valid) {
+        const uint32_t k = pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
+        const uint32_t at = pass == 0 ? i : __ldcg(position_in + i);
+        const uint32_t d = (k >> shift) & (bins - 1);
+        const unsigned peers = __match_any_sync(active, d);
+        const uint32_t place = mine[d] + __popc(peers & ((1u << lane) - 1));
+        __syncwarp(active);
+        if (lane == 31 - __clz(peers)) mine[d] = place + 1;
+        __stcg(key_out + place, k);
+        __stcg(position_out + place, at);
+      }
+      __syncwarp();
+    }
+    if (pass + 1 < p.passes) grid.sync();
+  }
+}
+
+// -------------------------------------------------------------------- sums
+constexpr int kChunkTokens = 32;  // a lane holds one
+constexpr int kSumThreads = 256;
+constexpr uint32_t kNoKey = 0xffffffffu;
+
+struct SumParams {
+  const uint32_t* key;
+  const uint32_t* position;
+  uint32_t n;
+  uint32_t rows;
+  uint32_t chunks;
+  uint32_t tiles;  // slices of the columns
+  const void* grad;
+  void* out;
+  float* partial;  // [2 * chunks][width]: a chunk's first run, its last
+  uint64_t width;
+  float scale;
+  int accumulate;
+};
+
+// A warp's slice of a row: kCols columns per lane, adjacent with kVector, else 32 apart.
+template <typename TG, bool kVector>
+struct Slice {
+  static constexpr int kCols = kVector ? 16 / static_cast<int>(sizeof(TG)) : 4;
+  uint64_t column;  // the lane's first
+  uint64_t width;
+  __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w) {
+    const int lane = threadIdx.x & 31;
+    column = static_cast<uint64_t>(tile) * (32 * kCols) + (kVector ? lane * kCols : lane);
+  }
+  // With kVector the width is a multiple of kCols: a lane has all of its columns or none.
+  template <typename T>
+  __device__ __forceinline__ void Load(const T* row, float* a) const {
+    if constexpr (kVector) {
+      if (column < width) LoadValues<T, kCols>(row + column, a);
+      else
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) a[e] = 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) a[e] = column + e * 32 < width ? ToAcc<float, T>(row[column + e * 32]) : 0.f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void Store(T* row, const float* a) const {
+    if constexpr (kVector) {
+      if (column < width) StoreValues<T, kCols>(row + column, a);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e)
+        if (column + e * 32 < width) row[column + e * 32] = FromAcc<T, float>(a[e]);
+    }
+  }
+};
+
+template <typename TO, typename S>
+__device__ __forceinline__ void WriteRow(const SumParams& p, const S& slice, uint32_t row, const float* sum) {
+  constexpr int kCols = S::kCols;
+  TO* out = static_cast<TO*>(p.out) + static_cast<uint64_t>(row) * p.width;
+  float v[kCols];
+  if (p.accumulate) {
+    slice.Load(out, v);
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) v[e] = fmaf(sum[e], p.scale, v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) v[e] = sum[e] * p.scale;
+  }
+  slice.Store(out, v);
+}
+
+template <typename TG, typename TO, bool kVector>
+__global__ void __launch_bounds__(kSumThreads) SumRunsKernel(SumParams p) {
+  using S = Slice<TG, kVector>;
+  constexpr int kCols = S::kCols, kAhead = 4;
+  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
+  if (item >= static_cast<uint64_t>(p.chunks) * p.tiles) return;
+  const uint32_t chunk = static_cast<uint32_t>(item / p.tiles);
+  const S slice(static_cast<uint32_t>(item - static_cast<uint64_t>(chunk) * p.tiles), p.width);
+  const int lane = threadIdx.x & 31;
+  const uint32_t i0 = chunk * kChunkTokens;
+  const int count = static_cast<int>(min(static_cast<uint32_t>(kChunkTokens), p.n - i0));
+  const uint32_t key = lane < count ? p.key[i0 + lane] : kNoKey;
+  const uint32_t position = lane < count ? p.position[i0 + lane] : 0;
+  const uint32_t before = i0 > 0 ? p.key[i0 - 1] : kNoKey;
+  const uint32_t behind = i0 + count < p.n ? p.key[i0 + count] : kNoKey;
+  const int known = __popc(__ballot_sync(0xffffffffu, key < p.rows));  // those without a row come last
+  const TG* grad = static_cast<const TG*>(p.grad);
+  float sum[kCols];
+#pragma unroll
+  for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+  bool first = true;  // the run that is being added began at the chunk's first token
+  for (int j = 0; j < known; j += kAhead) {
+    float a[kAhead][kCols];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (j + u < known) slice.Load(grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j + u)) * p.width, a[u]);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u >= known) break;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] += a[u][e];
+      const uint32_t k = __shfl_sync(0xffffffffu, key, j + u);
+      const uint32_t next = j + u + 1 < count ? __shfl_sync(0xffffffffu, key, (j + u + 1) & 31) : behind;
+      const bool last = j + u + 1 == count;
+      if (k == next && !last) continue;
+      const bool from_before = first && before == k;
+      if (from_before || (last && next == k)) {
+        slice.Store(p.partial + (2 * static_cast<uint64_t>(chunk) + (from_before ? 0 : 1)) * p.width, sum);
+      } else {
+        WriteRow<TO>(p, slice, k, sum);
+      }
+      first = false;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+    }
+  }
+}
+
+// The runs that go over a chunk's edge: the chunk in which a run begins adds its parts in order.
+template <typename TG, typename TO, bool kVector>
+__global__ void __launch_bounds__(kSumThreads) JoinRunsKernel(SumParams p) {
+  using S = Slice<TG, kVector>;
+  constexpr int kCols = S::kCols;
+  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
+  if (item >= static_cast<uint64_t>(p.chunks) * p.tiles) return;
+  const uint32_t chunk = static_cast<uint32_t>(item / p.tiles);
+  const uint32_t i0 = chunk * kChunkTokens;
+  if (p.n - i0 <= kChunkTokens) return;
+  const uint32_t k = p.key[i0 + kChunkTokens - 1];
+  if (k >= p.rows || p.key[i0 + kChunkTokens] != k) return;
+  if (p.key[i0] == k && i0 > 0 && p.key[i0 - 1] == k) return;  // it began in an earlier chunk
+  // The last token of the run.
+  uint32_t lo = i0 + kChunkTokens, hi = p.n;  // key[lo] == k, key[hi] != k
+  while (hi - lo > 1) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (p.key[mid] == k) lo = mid;
+    else hi = mid;
+  }
+  const uint32_t end = lo / kChunkTokens;
+  const S slice(static_cast<uint32_t>(item - static_cast<uint64_t>(chunk) * p.tiles), p.width);
+  float sum[kCols];
+  slice.Load(p.partial + (2 * static_cast<uint64_t>(chunk) + 1) * p.width, sum);
+#pragma unroll 4
+  for (uint32_t c = chunk + 1; c <= end; ++c) {
+    float a[kCols];
+    slice.Load(p.partial + 2 * static_cast<uint64_t>(c) * p.width, a);
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) sum[e] += a[e];
+  }
+  WriteRow<TO>(p, slice, k, sum);
+}
+
+}  // namespace dev
+
+namespace {
+
+template <typename TI, typename TO, bool kTokens64>
+cudaError_t LaunchLookup(const EmbeddingParams& p, cudaStream_t stream) {
+  constexpr int kN = dev::LookupQuantum<TI, TO>::kN;
+  auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
+  const bool vector = p.width % kN == 0 && aligned(p.weight, kN * sizeof(TI)) && aligned(p.out, kN * sizeof(TO));
+  const uint64_t per_row = vector ? p.width / kN : p.width;
+  const uint64_t quanta = p.num_tokens * per_row;
+  const uint64_t blocks = (quanta + dev::kLookupThreads - 1) / dev::kLookupThreads;
+  if (blocks > 0x7fffffffull || per_row > 0xffffffffull) return cudaErrorInvalidValue;
+  const TI* w = static_cast<const TI*>(p.weight);
+  TO* o = static_cast<TO*>(p.out);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  const uint32_t row = static_cast<uint32_t>(per_row);
+  if (vector) {
+    dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, quanta, row, p.rows, p.width, static_cast<float>(p.scale));
+  } else {
+    dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, quanta, row, p.rows, p.width, static_cast<float>(p.scale));
+  }
+  return cudaGetLastError();
+}
+
+// f(TI{}, TO{}) for a pair of the floating types that the embedding takes.
+template <typename TI, typename F>
+cudaError_t WithOutput(int dtype, F f) {
+  switch (static_cast<DType>(dtype)) {
+    case DType::kFloat32: return f(TI{}, float{});
+    case DType::kFloat16: return f(TI{}, __half{});
+    case DType::kBFloat16: return f(TI{}, __nv_bfloat16{});
+    default: return cudaErrorInvalidValue;
+  }
+}
+template <typename F>
+cudaError_t WithTypes(int dtype_in, int dtype_out, F f) {
+  switch (static_cast<DType>(dtype_in)) {
+    case DType::kFloat32: return WithOutput<float>(dtype_out, f);
+    case DType::kFloat16: return WithOutput<__half>(dtype_out, f);
+    case DType::kBFloat16: return WithOutput<__nv_bfloat16>(dtype_out, f);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+struct SortShape {
+  int passes, bits, blocks;
+  uint32_t per_block;
+};
+SortShape ShapeOf(uint64_t n, uint64_t rows) {
+  SortShape s;
+  int all = 1;  // bits of the keys, 0 .. rows
+  while (all < 32 && (rows >> all) != 0) ++all;
+  s.passes = (all + dev::kMostDigitBits - 1) / dev::kMostDigitBits;
+  s.bits = (all + s.passes - 1) / s.passes;
+  // A block takes at least 2048 tokens: with fewer the blocks' counts cost more than the tokens.
+  uint64_t blocks = std::min<uint64_t>(std::max<uint64_t>((n + 2047) / 2048, 1), dev::kMostSortBlocks);
+  uint64_t per = (n + blocks - 1) / blocks;
+  per = std::max<uint64_t>((per + dev::kSortThreads - 1) / dev::kSortThreads, 1) * dev::kSortThreads;
+  s.per_block = static_cast<uint32_t>(per);
+  s.blocks = static_cast<int>((n + per - 1) / per);
+  return s;
+}
+
+size_t Padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+}  // namespace
+
+cudaError_t LaunchEmbedding(const EmbeddingParams& p, cudaStream_t stream) {
+  if (p.num_tokens == 0 || p.width == 0) return cudaSuccess;
+  return WithTypes(p.dtype_weight, p.dtype_out, [&](auto ti, auto to) {
+    return p.tokens_are_64 ? LaunchLookup<decltype(ti), decltype(to), true>(p, stream) : LaunchLookup<decltype(ti), decltype(to), false>(p, stream);
+  });
+}
+
+size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
+  const SortShape s = ShapeOf(n, rows);
+  const uint64_t chunks = (n + dev::kChunkTokens - 1) / dev::kChunkTokens;
+  return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + 2 * chunks * width * 4;
+}
+
+cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t stream) {
+  if (p.rows == 0 || p.width == 0) return cudaSuccess;
+  if (p.num_tokens > 0x7fffffffull || p.rows > 0x7ffffffeull) return cudaErrorInvalidValue;
+  const size_t size_out = static_cast<DType>(p.dtype_out) == DType::kFloat32 ? 4 : 2;
+  if (!p.accumulate) {
+    const cudaError_t e = cudaMemsetAsync(p.out, 0, p.rows * p.width * size_out, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (p.num_tokens == 0) return cudaSuccess;
+  if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
+  const SortShape shape = ShapeOf(p.num_tokens, p.rows);
+  char* work = static_cast<char*>(p.work);
+  auto take = [&](size_t bytes) {
+    char* at = work;
+    work += Padded(bytes);
+    return at;
+  };
+  dev::SortParams sort{};
+  sort.tokens = p.tokens;
+  sort.tokens_are_64 = p.tokens_are_64;
+  sort.n = static_cast<uint32_t>(p.num_tokens);
+  sort.rows = static_cast<uint32_t>(p.rows);
+  sort.padding = p.padding;
+  sort.per_block = shape.per_block;
+  sort.passes = shape.passes;
+  sort.bits = shape.bits;
+  for (int i = 0; i < 2; ++i) {
+    sort.key[i] = reinterpret_cast<uint32_t*>(take(p.num_tokens * 4));
+    sort.position[i] = reinterpret_cast<uint32_t*>(take(p.num_tokens * 4));
+  }
+  sort.counts = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(shape.blocks) << shape.bits << 2));
+  const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
+  cudaError_t e = AllowSharedMemory(dev::SortTokensKernel, smem);
+  if (e != cudaSuccess) return e;
+  void* args[] = {&sort};
+  e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&dev::SortTokensKernel), dim3(static_cast<unsigned>(shape.blocks)), dim3(dev::kSortThreads), args,
+                                  smem, stream);
+  if (e != cudaSuccess) return e;
+  dev::SumParams sum{};
+  const int last = (shape.passes - 1) & 1;
+  sum.key = sort.key[last];
+  sum.position = sort.position[last];
+  sum.n = sort.n;
+  sum.rows = sort.rows;
+  sum.chunks = (sort.n + dev::kChunkTokens - 1) / dev::kChunkTokens;
+  sum.grad = p.grad;
+  sum.out = p.out;
+  sum.partial = reinterpret_cast<float*>(work);
+  sum.width = p.width;
+  sum.scale = static_cast<float>(p.scale);
+  sum.accumulate = p.accumulate ? 1 : 0;
+  return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
+    using TG = decltype(tg);
+    using TO = decltype(to);
+    constexpr uint64_t kCols = dev::Slice<TG, true>::kCols;
+    auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
+    const bool vector = p.width % kCols == 0 && aligned(p.grad, 16) && aligned(p.out, kCols * sizeof(TO));
+    const uint64_t tile = 32 * (vector ? kCols : dev::Slice<TG, false>::kCols);
+    const uint64_t tiles = (p.width + tile - 1) / tile;
+    const uint64_t blocks = (sum.chunks * tiles + dev::kSumThreads / 32 - 1) / (dev::kSumThreads / 32);
+    if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+    sum.tiles = static_cast<uint32_t>(tiles);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    if (vector) {
+      dev::SumRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
+      if (sum.chunks > 1) dev::JoinRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
+    } else {
+      dev::SumRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
+      if (sum.chunks > 1) dev::JoinRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
+    }
+    return cudaGetLastError();
+  });
+}
+
+}  // namespace ibcomm

@@ -1,5 +1,7 @@
 #include "ibcomm/c_api.h"
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -11,6 +13,7 @@
 #ifdef USE_CUDA
 #include <cuda_runtime.h>
 
+#include "grad_ops.h"
 #include "ibcomm/emu_world.h"
 #include "kernels.h"
 #endif
@@ -81,6 +84,103 @@ void NeedHandle(const void* h) {
 #ifndef USE_CUDA
   IBCOMM_FAIL(NOT_SUPPORTED, "This build of the library has no CUDA support.\n");
 #endif
+}
+
+using ibcomm::DType;
+
+bool Floating(int d) {
+  const DType t = CheckDType(d);
+  return t != DType::kInt32 && t != DType::kInt64;
+}
+
+// Memory that a call writes must be read or written nowhere else in the call.
+struct Stretch {
+  uintptr_t begin, end;
+  bool written;
+  bool operator<(const Stretch& o) const { return begin < o.begin; }
+};
+void CheckApart(std::vector<Stretch>* all) {
+  if (!std::is_sorted(all->begin(), all->end())) std::sort(all->begin(), all->end());
+  uintptr_t read = 0, written = 0;  // how far those before reach
+  for (const Stretch& s : *all) {
+    if (s.begin < written || (s.written && s.begin < read))
+      IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors that are written must not share memory with another tensor of the call.\n");
+    uintptr_t& reach = s.written ? written : read;
+    reach = std::max(reach, s.end);
+  }
+}
+
+void CheckGradTensors(const ibcomm_grad_tensor* tensors, int count, int power, bool clip, bool host) {
+  if (count < 0 || (count > 0 && tensors == nullptr)) IBCOMM_FAIL(INVALID_ARGUMENT, "The list of tensors is null.\n");
+  if (power != 0 && power != 2) IBCOMM_FAIL(NOT_SUPPORTED, "The norm's power is 2 or 0 (the maximum), got %d.\n", power);
+  std::vector<Stretch> all;
+  if (clip) all.reserve(2 * static_cast<size_t>(count));
+  for (int i = 0; i < count; ++i) {
+    const ibcomm_grad_tensor& t = tensors[i];
+    if (!Floating(t.dtype_in) || (host && DTypeSize(CheckDType(t.dtype_in)) < 4))
+      IBCOMM_FAIL(NOT_SUPPORTED, "No norm of %s tensors%s.\n", DTypeName(CheckDType(t.dtype_in)), host ? " on the host" : "");
+    const size_t size = DTypeSize(CheckDType(t.dtype_in));
+    if (t.len_elements == 0) continue;
+    if (t.in == nullptr || reinterpret_cast<uintptr_t>(t.in) % size != 0) IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must have memory, aligned to their type.\n");
+    if (!clip) continue;
+    const DType a = CheckDType(t.dtype_in), b = CheckDType(t.dtype_out);
+    const bool pair = a == b || (!host && ((a == DType::kFloat32 && (b == DType::kFloat16 || b == DType::kBFloat16)) ||
+                                           (b == DType::kFloat32 && (a == DType::kFloat16 || a == DType::kBFloat16))));
+    if (!pair) IBCOMM_FAIL(NOT_SUPPORTED, "No clipping of %s into %s.\n", DTypeName(a), DTypeName(b));
+    if (t.out == nullptr || reinterpret_cast<uintptr_t>(t.out) % DTypeSize(b) != 0) IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must have memory, aligned to their type.\n");
+    const uintptr_t in = reinterpret_cast<uintptr_t>(t.in), out = reinterpret_cast<uintptr_t>(t.out);
+    all.push_back({out, out + t.len_elements * DTypeSize(b), true});
+    if (in != out || a != b) all.push_back({in, in + t.len_elements * size, false});
+  }
+  if (clip) CheckApart(&all);
+}
+
+template <typename T>
+double HostSum(const T* x, size_t n, int power) {
+  double s = 0.0;
+  for (size_t i = 0; i < n; ++i) {
+    const double v = std::fabs(static_cast<double>(x[i]));
+    if (power == 2) s += v * v;
+    else if (!(v <= s) && !std::isnan(s)) s = v;
+  }
+  return s;
+}
+template <typename T>
+void HostScale(const T* in, T* out, size_t n, double coefficient) {
+  const T c = static_cast<T>(coefficient);
+  for (size_t i = 0; i < n; ++i) out[i] = in[i] * c;
+}
+
+#ifdef USE_CUDA
+std::vector<ibcomm::GradTensor> GradTensors(const ibcomm_grad_tensor* tensors, int count) {
+  std::vector<ibcomm::GradTensor> list(static_cast<size_t>(count));
+  for (int i = 0; i < count; ++i) list[i] = {tensors[i].in, tensors[i].out, tensors[i].len_elements, tensors[i].dtype_in, tensors[i].dtype_out};
+  return list;
+}
+#endif
+
+void CheckSums(const double* sums, int num_sums, const double* work, int norm_dtype) {
+  if (sums != nullptr ? num_sums < 1 : work == nullptr) IBCOMM_FAIL(INVALID_ARGUMENT, "There are neither sums nor a workspace.\n");
+  const DType t = CheckDType(norm_dtype);
+  if (t != DType::kFloat32 && t != DType::kFloat64) IBCOMM_FAIL(NOT_SUPPORTED, "A norm is float32 or float64.\n");
+}
+
+void CheckEmbedding(const void* tokens, int tokens_dtype, size_t num_tokens, size_t rows, size_t width, const void* table, int table_dtype, const void* values,
+                    int values_dtype, double scale) {
+  const DType t = CheckDType(tokens_dtype);
+  if (t != DType::kInt32 && t != DType::kInt64) IBCOMM_FAIL(NOT_SUPPORTED, "Tokens are int32 or int64, got %s.\n", DTypeName(t));
+  for (int d : {table_dtype, values_dtype})
+    if (!Floating(d) || CheckDType(d) == DType::kFloat64) IBCOMM_FAIL(NOT_SUPPORTED, "No embedding of %s.\n", DTypeName(CheckDType(d)));
+  if (num_tokens > 0x7fffffffull || rows > 0x7ffffffeull || width > 0x7fffffffull)
+    IBCOMM_FAIL(NOT_SUPPORTED, "Tokens, rows and their width are counted in 31 bits.\n");
+  if ((num_tokens > 0 && tokens == nullptr) || (num_tokens > 0 && width > 0 && values == nullptr) || (rows > 0 && width > 0 && table == nullptr))
+    IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must have memory.\n");
+  if (std::isnan(scale)) IBCOMM_FAIL(INVALID_ARGUMENT, "The scale is not a number.\n");
+}
+
+Stretch Memory(const void* p, size_t elements, int dtype, bool written) {
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
+  return {begin, begin + elements * DTypeSize(static_cast<DType>(dtype)), written};
 }
 
 }  // namespace
@@ -576,6 +676,122 @@ int ibcomm_copy_scale(const void* in, void* out, size_t n, int dtype_in, int dty
     if (e != cudaSuccess) IBCOMM_FAIL(CUDA_ERROR, "copy kernel launch failed: %s\n", cudaGetErrorString(e));
 #else
     (void)in; (void)out; (void)n; (void)dtype_in; (void)dtype_out; (void)scale; (void)stream;
+#endif
+  });
+}
+
+int ibcomm_grad_norm(const ibcomm_grad_tensor* tensors, int count, int power, const double* sums, int num_sums, double* work, void* norm,
+                     int norm_dtype, double* sum, void* stream) {
+  return Guard([&] {
+    NeedCuda();
+    CheckGradTensors(tensors, count, power, false, false);
+    CheckSums(sums, num_sums, work, norm_dtype);
+#ifdef USE_CUDA
+    const std::vector<ibcomm::GradTensor> list = GradTensors(tensors, count);
+    const ibcomm::GradNormParams p{list.data(), count, static_cast<ibcomm::GradPower>(power), work, sums, num_sums, norm, norm_dtype == 1, sum, false, 0.0};
+    cudaError_t e = ibcomm::LaunchGradNorm(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) IBCOMM_FAIL(CUDA_ERROR, "gradient norm launch failed: %s\n", cudaGetErrorString(e));
+#else
+    (void)norm; (void)sum; (void)stream;
+#endif
+  });
+}
+
+int ibcomm_clip_grads(const ibcomm_grad_tensor* tensors, int count, int power, double max_norm, const double* sums, int num_sums, double* work,
+                      void* norm, int norm_dtype, void* stream) {
+  return Guard([&] {
+    NeedCuda();
+    CheckGradTensors(tensors, count, power, true, false);
+    CheckSums(sums, num_sums, work, norm_dtype);
+    if (!(max_norm >= 0.0)) IBCOMM_FAIL(INVALID_ARGUMENT, "The largest norm is negative or not a number.\n");
+#ifdef USE_CUDA
+    const std::vector<ibcomm::GradTensor> list = GradTensors(tensors, count);
+    const ibcomm::GradNormParams p{list.data(), count, static_cast<ibcomm::GradPower>(power), work, sums, num_sums, norm, norm_dtype == 1, nullptr, true, max_norm};
+    cudaError_t e = ibcomm::LaunchGradNorm(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) IBCOMM_FAIL(CUDA_ERROR, "clipping launch failed: %s\n", cudaGetErrorString(e));
+#else
+    (void)norm; (void)stream;
+#endif
+  });
+}
+
+int ibcomm_grad_sum_host(const ibcomm_grad_tensor* tensors, int count, int power, double* sum) {
+  return Guard([&] {
+    CheckGradTensors(tensors, count, power, false, true);
+    if (sum == nullptr) IBCOMM_FAIL(INVALID_ARGUMENT, "sum is null.\n");
+    double total = 0.0;
+    for (int i = 0; i < count; ++i) {
+      const ibcomm_grad_tensor& t = tensors[i];
+      const double s = static_cast<DType>(t.dtype_in) == DType::kFloat32 ? HostSum(static_cast<const float*>(t.in), t.len_elements, power)
+                                                                         : HostSum(static_cast<const double*>(t.in), t.len_elements, power);
+      if (power == 2) total += s;
+      else if (!(s <= total) && !std::isnan(total)) total = s;
+    }
+    *sum = total;
+  });
+}
+
+int ibcomm_scale_grads_host(const ibcomm_grad_tensor* tensors, int count, double coefficient) {
+  return Guard([&] {
+    CheckGradTensors(tensors, count, 2, true, true);
+    for (int i = 0; i < count; ++i) {
+      const ibcomm_grad_tensor& t = tensors[i];
+      if (static_cast<DType>(t.dtype_in) == DType::kFloat32) HostScale(static_cast<const float*>(t.in), static_cast<float*>(t.out), t.len_elements, coefficient);
+      else HostScale(static_cast<const double*>(t.in), static_cast<double*>(t.out), t.len_elements, coefficient);
+    }
+  });
+}
+
+int ibcomm_embedding(const void* tokens, int tokens_dtype, size_t num_tokens, const void* weight, int weight_dtype, size_t rows, size_t width,
+                     void* out, int out_dtype, double scale, void* stream) {
+  return Guard([&] {
+    NeedCuda();
+    CheckEmbedding(tokens, tokens_dtype, num_tokens, rows, width, weight, weight_dtype, out, out_dtype, scale);
+    std::vector<Stretch> all{Memory(tokens, num_tokens, tokens_dtype, false), Memory(weight, rows * width, weight_dtype, false),
+                             Memory(out, num_tokens * width, out_dtype, true)};
+    CheckApart(&all);
+#ifdef USE_CUDA
+    const ibcomm::EmbeddingParams p{tokens, tokens_dtype == 3, num_tokens, weight, rows, width, weight_dtype, out, out_dtype, scale};
+    cudaError_t e = ibcomm::LaunchEmbedding(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) IBCOMM_FAIL(CUDA_ERROR, "embedding launch failed: %s\n", cudaGetErrorString(e));
+#else
+    (void)stream;
+#endif
+  });
+}
+
+int ibcomm_embedding_grad_work(size_t num_tokens, size_t rows, size_t width, size_t* bytes) {
+  return Guard([&] {
+    NeedCuda();
+    if (bytes == nullptr) IBCOMM_FAIL(INVALID_ARGUMENT, "bytes is null.\n");
+#ifdef USE_CUDA
+    *bytes = ibcomm::EmbeddingGradWorkBytes(num_tokens, rows, width);
+#else
+    (void)num_tokens; (void)rows; (void)width;
+#endif
+  });
+}
+
+int ibcomm_embedding_grad(const void* tokens, int tokens_dtype, size_t num_tokens, const void* grad, int grad_dtype, void* out, int out_dtype,
+                          size_t rows, size_t width, int64_t padding_row, double scale, int accumulate, void* work, size_t work_bytes,
+                          void* stream) {
+  return Guard([&] {
+    NeedCuda();
+    CheckEmbedding(tokens, tokens_dtype, num_tokens, rows, width, out, out_dtype, grad, grad_dtype, scale);
+    std::vector<Stretch> all{Memory(tokens, num_tokens, tokens_dtype, false), Memory(grad, num_tokens * width, grad_dtype, false),
+                             Memory(out, rows * width, out_dtype, true)};
+    CheckApart(&all);
+    if (padding_row < -1 || padding_row >= static_cast<int64_t>(rows)) IBCOMM_FAIL(INVALID_ARGUMENT, "The padding row is no row of the table.\n");
+#ifdef USE_CUDA
+    const size_t need = ibcomm::EmbeddingGradWorkBytes(num_tokens, rows, width);
+    if (work_bytes < need || (need > 0 && reinterpret_cast<uintptr_t>(work) % 256 != 0) || (need > 0 && work == nullptr))
+      IBCOMM_FAIL(INVALID_ARGUMENT, "The workspace has %zu bytes of the %zu needed, or misses its boundary of 256 bytes.\n", work_bytes, need);
+    const ibcomm::EmbeddingGradParams p{tokens, tokens_dtype == 3, num_tokens, grad,       grad_dtype, out,  out_dtype,
+                                        rows,   width,             padding_row, scale, accumulate != 0, work, work_bytes};
+    cudaError_t e = ibcomm::LaunchEmbeddingGrad(p, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) IBCOMM_FAIL(CUDA_ERROR, "embedding gradient launch failed: %s\n", cudaGetErrorString(e));
+#else
+    (void)padding_row; (void)accumulate; (void)work; (void)work_bytes; (void)stream;
 #endif
   });
 }

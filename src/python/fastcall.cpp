@@ -13,9 +13,14 @@
 // them into the Python exceptions torch's own methods raise.
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <utility>
+#include <vector>
 
 #include "ibcomm/c_api.h"
 #include "ibcomm/device_types.h"
@@ -275,12 +280,254 @@ PyObject* EmuRsAg(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The tensors of a list as the norm and clipping take them: dense, on one GPU.  It
+// holds on to the sequences, like RankTensors.
+struct GradList {
+  PyObject* in = nullptr;
+  PyObject* out = nullptr;
+  std::vector<ibcomm_grad_tensor> tensors;
+  c10::Device device{c10::DeviceType::CUDA, 0};
+  bool any_double = false;
+
+  GradList() = default;
+  GradList(const GradList&) = delete;
+  GradList& operator=(const GradList&) = delete;
+  ~GradList() {
+    Py_XDECREF(in);
+    Py_XDECREF(out);
+  }
+
+  static const at::Tensor* Dense(PyObject* o, int* dtype) {
+    if (!THPVariable_Check(o)) {
+      PyErr_SetString(PyExc_TypeError, "a torch.Tensor is expected");
+      return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(o);
+    *dtype = DTypeCode(t.scalar_type());
+    if (*dtype < 0) {
+      Raise(kNotSupported, (std::string("unsupported dtype ") + c10::toString(t.scalar_type())).c_str());
+      return nullptr;
+    }
+    if (!t.is_cuda()) {
+      Raise(kInvalidArgument, "tensors must live on the GPU");
+      return nullptr;
+    }
+    // The order of the elements does not matter, only that nothing lies between them.
+    if (t.layout() != c10::kStrided || !(t.is_contiguous() || t.is_non_overlapping_and_dense())) {
+      Raise(kInvalidArgument, "tensors must be dense");
+      return nullptr;
+    }
+    return &t;
+  }
+
+  // `outs`: None for the norm alone, the same sequence for clipping in place.
+  bool Read(PyObject* ins, PyObject* outs) {
+    in = PySequence_Fast(ins, "a sequence of tensors is expected");
+    if (in == nullptr) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(in);
+    const bool clip = outs != Py_None, in_place = outs == ins;
+    if (n == 0) {
+      Raise(kInvalidArgument, "a tensor is expected at least");
+      return false;
+    }
+    if (clip && !in_place) {
+      out = PySequence_Fast(outs, "a sequence of tensors is expected");
+      if (out == nullptr) return false;
+      if (PySequence_Fast_GET_SIZE(out) != n) {
+        Raise(kInvalidArgument, "one output per tensor is expected");
+        return false;
+      }
+    }
+    tensors.resize(static_cast<size_t>(n));
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      ibcomm_grad_tensor& g = tensors[static_cast<size_t>(i)];
+      const at::Tensor* t = Dense(PySequence_Fast_GET_ITEM(in, i), &g.dtype_in);
+      if (t == nullptr) return false;
+      if (i == 0) device = t->device();
+      g.len_elements = static_cast<size_t>(t->numel());
+      any_double = any_double || g.dtype_in == 1;
+      g.in = t->const_data_ptr();
+      g.out = nullptr;
+      g.dtype_out = g.dtype_in;
+      const at::Tensor* o = t;
+      if (clip && !in_place) {
+        o = Dense(PySequence_Fast_GET_ITEM(out, i), &g.dtype_out);
+        if (o == nullptr) return false;
+        if (o->sizes() != t->sizes() || !(o->strides() == t->strides() || (o->is_contiguous() && t->is_contiguous()))) {
+          Raise(kInvalidArgument, "an output must match its tensor in shape and strides");
+          return false;
+        }
+      }
+      if (t->device() != device || o->device() != device) {
+        Raise(kInvalidArgument, "the tensors must live on one GPU");
+        return false;
+      }
+      if (clip) g.out = o->data_ptr();
+    }
+    return true;
+  }
+};
+
+// Device memory of this call; freed into the current stream's pool.
+at::Tensor Empty(at::IntArrayRef sizes, c10::ScalarType type, c10::Device device) {
+  return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+}
+
+// The ranks' sums (float64, on the list's GPU), or None.
+bool ToSums(PyObject* o, const GradList& list, const double** sums, int* count) {
+  *sums = nullptr;
+  *count = 0;
+  if (o == Py_None) return true;
+  int d;
+  const at::Tensor* t = Tensor(o, &d);
+  if (t == nullptr) return false;
+  if (d != 1 || t->device() != list.device || t->numel() < 1 || t->numel() > (1 << 20)) {
+    Raise(kInvalidArgument, "the ranks' sums must be float64 on the tensors' GPU");
+    return false;
+  }
+  *sums = static_cast<const double*>(t->const_data_ptr());
+  *count = static_cast<int>(t->numel());
+  return true;
+}
+
+// grad_norm(tensors, power, sums, want_sum) -> the norm, or with want_sum the sum that ranks have to join (float64, one element)
+PyObject* GradNorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!WantArgs(n, 4)) return nullptr;
+  GradList list;
+  if (!list.Read(a[0], Py_None)) return nullptr;
+  const int power = static_cast<int>(PyLong_AsLong(a[1]));
+  const int want_sum = static_cast<int>(PyLong_AsLong(a[3]));
+  const double* sums;
+  int num_sums;
+  if (PyErr_Occurred() || !ToSums(a[2], list, &sums, &num_sums)) return nullptr;
+  const c10::cuda::CUDAGuard guard(list.device);
+  at::Tensor work = Empty({IBCOMM_NORM_WORK}, c10::kDouble, list.device);
+  at::Tensor result = want_sum ? Empty({1}, c10::kDouble, list.device) : Empty({}, list.any_double ? c10::kDouble : c10::kFloat, list.device);
+  void* stream = c10::cuda::getCurrentCUDAStream(list.device.index()).stream();
+  void* norm = want_sum ? nullptr : result.data_ptr();
+  double* sum = want_sum ? static_cast<double*>(result.data_ptr()) : nullptr;
+  double* w = static_cast<double*>(work.data_ptr());
+  int code;
+  Py_BEGIN_ALLOW_THREADS;
+  code = ibcomm_grad_norm(list.tensors.data(), static_cast<int>(list.tensors.size()), power, sums, num_sums, w, norm, list.any_double ? 1 : 0, sum, stream);
+  Py_END_ALLOW_THREADS;
+  if (code != 0) return RaiseLast(code);
+  return THPVariable_Wrap(std::move(result));
+  END_HANDLE_TH_ERRORS
+}
+
+// clip_grads(tensors, outs, power, max_norm, sums) -> the norm; outs None: in place
+PyObject* ClipGrads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!WantArgs(n, 5)) return nullptr;
+  GradList list;
+  if (!list.Read(a[0], a[1] == Py_None ? a[0] : a[1])) return nullptr;
+  const int power = static_cast<int>(PyLong_AsLong(a[2]));
+  const double max_norm = PyFloat_AsDouble(a[3]);
+  const double* sums;
+  int num_sums;
+  if (PyErr_Occurred() || !ToSums(a[4], list, &sums, &num_sums)) return nullptr;
+  const c10::cuda::CUDAGuard guard(list.device);
+  at::Tensor work = Empty({IBCOMM_NORM_WORK}, c10::kDouble, list.device);
+  at::Tensor result = Empty({}, list.any_double ? c10::kDouble : c10::kFloat, list.device);
+  void* stream = c10::cuda::getCurrentCUDAStream(list.device.index()).stream();
+  void* norm = result.data_ptr();
+  double* w = static_cast<double*>(work.data_ptr());
+  int code;
+  Py_BEGIN_ALLOW_THREADS;
+  code = ibcomm_clip_grads(list.tensors.data(), static_cast<int>(list.tensors.size()), power, max_norm, sums, num_sums, w, norm, list.any_double ? 1 : 0, stream);
+  Py_END_ALLOW_THREADS;
+  if (code != 0) return RaiseLast(code);
+  return THPVariable_Wrap(std::move(result));
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding(tokens, weight, out_dtype, scale) -> rows; out_dtype < 0: the table's type
+PyObject* Embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!WantArgs(n, 4)) return nullptr;
+  int dt, dw;
+  const at::Tensor* tokens = Tensor(a[0], &dt);
+  if (tokens == nullptr) return nullptr;
+  const at::Tensor* weight = Tensor(a[1], &dw);
+  if (weight == nullptr) return nullptr;
+  const int wanted = static_cast<int>(PyLong_AsLong(a[2]));
+  const double scale = PyFloat_AsDouble(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (weight->dim() != 2) return Raise(kInvalidArgument, "a table has rows and columns");
+  if (!tokens->is_cuda() || !weight->is_cuda() || tokens->device() != weight->device())
+    return Raise(kInvalidArgument, "tokens and table must live on the same GPU");
+  const int out_dtype = wanted < 0 ? dw : wanted;
+  if (out_dtype != 0 && out_dtype != 4 && out_dtype != 5) return Raise(kNotSupported, "rows are float32, float16 or bfloat16");
+  const c10::Device device = weight->device();
+  const c10::cuda::CUDAGuard guard(device);
+  c10::SmallVector<int64_t, 8> sizes(tokens->sizes().begin(), tokens->sizes().end());
+  sizes.push_back(weight->size(1));
+  at::Tensor out = Empty(sizes, out_dtype == 0 ? c10::kFloat : out_dtype == 4 ? c10::kHalf : c10::kBFloat16, device);
+  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  const void* t = tokens->const_data_ptr();
+  const void* w = weight->const_data_ptr();
+  void* o = out.data_ptr();
+  const size_t count = static_cast<size_t>(tokens->numel()), rows = static_cast<size_t>(weight->size(0)), width = static_cast<size_t>(weight->size(1));
+  int code;
+  Py_BEGIN_ALLOW_THREADS;
+  code = ibcomm_embedding(t, dt, count, w, dw, rows, width, o, out_dtype, scale, stream);
+  Py_END_ALLOW_THREADS;
+  if (code != 0) return RaiseLast(code);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding_grad(tokens, grad, out, padding_row, scale, accumulate)
+PyObject* EmbeddingGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!WantArgs(n, 6)) return nullptr;
+  int dt, dg, dout;
+  const at::Tensor* tokens = Tensor(a[0], &dt);
+  if (tokens == nullptr) return nullptr;
+  const at::Tensor* grad = Tensor(a[1], &dg);
+  if (grad == nullptr) return nullptr;
+  const at::Tensor* out = Tensor(a[2], &dout);
+  if (out == nullptr) return nullptr;
+  const int64_t padding = PyLong_AsLongLong(a[3]);
+  const double scale = PyFloat_AsDouble(a[4]);
+  const int accumulate = PyObject_IsTrue(a[5]);
+  if (PyErr_Occurred()) return nullptr;
+  if (out->dim() != 2) return Raise(kInvalidArgument, "a table has rows and columns");
+  const size_t count = static_cast<size_t>(tokens->numel()), rows = static_cast<size_t>(out->size(0)), width = static_cast<size_t>(out->size(1));
+  if (grad->dim() < 1 || grad->size(-1) != out->size(1) || static_cast<size_t>(grad->numel()) != count * width)
+    return Raise(kInvalidArgument, "grad must hold a row of the table's width for every token");
+  if (!tokens->is_cuda() || !grad->is_cuda() || !out->is_cuda() || tokens->device() != out->device() || grad->device() != out->device())
+    return Raise(kInvalidArgument, "tokens, grad and table must live on the same GPU");
+  const c10::Device device = out->device();
+  const c10::cuda::CUDAGuard guard(device);
+  size_t bytes = 0;
+  int code = ibcomm_embedding_grad_work(count, rows, width, &bytes);
+  if (code != 0) return RaiseLast(code);
+  at::Tensor work = Empty({static_cast<int64_t>(bytes)}, c10::kByte, device);
+  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  const void* t = tokens->const_data_ptr();
+  const void* g = grad->const_data_ptr();
+  void* o = out->data_ptr();
+  void* w = work.data_ptr();
+  Py_BEGIN_ALLOW_THREADS;
+  code = ibcomm_embedding_grad(t, dt, count, g, dg, o, dout, rows, width, padding, scale, accumulate, w, bytes, stream);
+  Py_END_ALLOW_THREADS;
+  return Done(code);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"set_error", SetError, METH_O, "set_error(exception_class)"},
     {"allreduce", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Allreduce)), METH_FASTCALL, nullptr},
     {"copy_scale", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(CopyScale)), METH_FASTCALL, nullptr},
     {"emu_allreduce", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(EmuAllreduce)), METH_FASTCALL, nullptr},
     {"emu_rsag", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(EmuRsAg)), METH_FASTCALL, nullptr},
+    {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(GradNorm)), METH_FASTCALL, nullptr},
+    {"clip_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(ClipGrads)), METH_FASTCALL, nullptr},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(Embedding)), METH_FASTCALL, nullptr},
+    {"embedding_grad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(EmbeddingGrad)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
