@@ -2,12 +2,12 @@
 // table: out[v] (+)= round(scale * sum of grad[t] over the tokens t that name v).
 //
 // The gradient sorts the tokens' positions by row (a stable radix sort, so that
-// the positions of a row stay in their order), cuts the sorted list into chunks
-// of kChunkTokens and gives every warp a chunk and a slice of the columns.  The
-// warp adds the rows of a run of equal tokens in fp32 registers; a run inside
-// the chunk is written at once, one that a chunk's edge cuts leaves partial sums
-// in the workspace, which a second kernel adds in the chunks' order.  No atomics
-// on values: the result does not depend on the order of execution.
+// the positions of a row stay in their order), cuts the sorted list into ranges
+// and gives every block a range and a slice of the columns.  Its warps add the
+// rows of a run of equal tokens in fp32 registers; a run inside a warp's part is
+// written at once, one over its edges is joined in shared memory, one over the
+// range's edges in the workspace by the block that arrives last.  Every sum is
+// added in the tokens' order: the result does not depend on that of execution.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -106,6 +106,8 @@ struct SortParams {
   uint32_t* key[2];
   uint32_t* position[2];
   uint32_t* counts;    // gridDim.x x bins
+  uint32_t* zeros;     // to be cleared for the kernel behind
+  uint32_t num_zeros;
 };
 
 __device__ __forceinline__ uint32_t KeyOf(const SortParams& p, uint32_t t) {
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
   const uint32_t begin = blockIdx.x * p.per_block + warp * part;
   const uint32_t end = min(begin + part, p.n);
   uint32_t* mine = warp_counts + warp * bins;
+  for (uint32_t i = blockIdx.x * kSortThreads + threadIdx.x; i < p.num_zeros; i += gridDim.x * kSortThreads) p.zeros[i] = 0;
   for (int pass = 0; pass < p.passes; ++pass) {
     const uint32_t* key_in = p.key[(pass + 1) & 1];
     const uint32_t* position_in = p.position[(pass + 1) & 1];
@@ -203,8 +206,10 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 }
 
 // -------------------------------------------------------------------- sums
-constexpr int kChunkTokens = 32;  // a lane holds one
-constexpr int kSumThreads = 256;
+constexpr int kSumWarps = 8;
+constexpr int kSumThreads = 32 * kSumWarps;
+constexpr int kMostWarpTokens = 16;
+constexpr int kAhead = 8;  // rows in flight per warp
 constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct SumParams {
@@ -212,11 +217,13 @@ struct SumParams {
   const uint32_t* position;
   uint32_t n;
   uint32_t rows;
-  uint32_t chunks;
-  uint32_t tiles;  // slices of the columns
+  uint32_t per_warp;  // tokens, 32 at most
+  uint32_t ranges;    // of kSumWarps * per_warp tokens
+  uint32_t tiles;     // slices of the columns
   const void* grad;
   void* out;
-  float* partial;  // [2 * chunks][width]: a chunk's first run, its last
+  float* partial;     // [2 * ranges][width]: a range's run that began before it, the one that goes on behind it
+  uint32_t* arrived;  // [ranges][tiles], zero
   uint64_t width;
   float scale;
   int accumulate;
@@ -226,6 +233,10 @@ struct SumParams {
 template <typename TG, bool kVector>
 struct Slice {
   static constexpr int kCols = kVector ? 16 / static_cast<int>(sizeof(TG)) : 4;
+  struct Raw {
+    uint4 v;
+    TG e[kVector ? 1 : kCols];
+  };
   uint64_t column;  // the lane's first
   uint64_t width;
   __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w) {
@@ -233,13 +244,32 @@ struct Slice {
     column = static_cast<uint64_t>(tile) * (32 * kCols) + (kVector ? lane * kCols : lane);
   }
   // With kVector the width is a multiple of kCols: a lane has all of its columns or none.
+  __device__ __forceinline__ void LoadRaw(const TG* row, Raw* r) const {
+    if constexpr (kVector) {
+      if (column < width) r->v = Ld16(row + column);
+      else r->v = make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) r->e[e] = column + e * 32 < width ? row[column + e * 32] : FromAcc<TG, float>(0.f);
+    }
+  }
+  __device__ __forceinline__ static void AddRaw(const Raw& r, float* sum) {
+    if constexpr (kVector) {
+      VecIO<TG>::Add(r.v, sum);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] += ToAcc<float, TG>(r.e[e]);
+    }
+  }
   template <typename T>
   __device__ __forceinline__ void Load(const T* row, float* a) const {
     if constexpr (kVector) {
-      if (column < width) LoadValues<T, kCols>(row + column, a);
-      else
+      if (column < width) {
+        LoadValues<T, kCols>(row + column, a);
+      } else {
 #pragma unroll
         for (int e = 0; e < kCols; ++e) a[e] = 0.f;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < kCols; ++e) a[e] = column + e * 32 < width ? ToAcc<float, T>(row[column + e * 32]) : 0.f;
@@ -255,6 +285,22 @@ struct Slice {
         if (column + e * 32 < width) row[column + e * 32] = FromAcc<T, float>(a[e]);
     }
   }
+  // Added by the memory: nothing to wait for.  Only one warp adds to a row, once.
+  __device__ __forceinline__ void Add(float* row, const float* a) const {
+    if constexpr (kVector) {
+      if (column < width) {
+#pragma unroll
+        for (int e = 0; e < kCols; e += 4)
+          asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + column + e), "f"(a[e]), "f"(a[e + 1]), "f"(a[e + 2]),
+                       "f"(a[e + 3])
+                       : "memory");
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e)
+        if (column + e * 32 < width) atomicAdd(row + column + e * 32, a[e]);
+    }
+  }
 };
 
 template <typename TO, typename S>
@@ -262,97 +308,170 @@ __device__ __forceinline__ void WriteRow(const SumParams& p, const S& slice, uin
   constexpr int kCols = S::kCols;
   TO* out = static_cast<TO*>(p.out) + static_cast<uint64_t>(row) * p.width;
   float v[kCols];
-  if (p.accumulate) {
-    slice.Load(out, v);
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) v[e] = fmaf(sum[e], p.scale, v[e]);
+  for (int e = 0; e < kCols; ++e) v[e] = sum[e] * p.scale;
+  if (!p.accumulate) {
+    slice.Store(out, v);
+  } else if constexpr (sizeof(TO) == 4) {
+    slice.Add(out, v);
   } else {
+    float old[kCols];
+    slice.Load(out, old);
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) v[e] = sum[e] * p.scale;
+    for (int e = 0; e < kCols; ++e) v[e] += old[e];
+    slice.Store(out, v);
   }
-  slice.Store(out, v);
 }
 
+// The first and last range of the run of `k` that goes over an edge of `range`.
+__device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint32_t range, uint32_t* first, uint32_t* last) {
+  const uint32_t lane = threadIdx.x & 31, per = p.per_warp * kSumWarps;
+  // Whether the run goes over the edge between range b - 1 and range b.
+  auto crosses = [&](uint32_t b) { return b >= 1 && b < p.ranges && p.key[b * per - 1] == k && p.key[b * per] == k; };
+  uint32_t c = range;
+  for (;;) {
+    const unsigned m = __ballot_sync(0xffffffffu, c >= lane && crosses(c - lane));
+    const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+    c -= run;
+    if (run < 32) break;
+  }
+  *first = c;
+  c = range;
+  for (;;) {
+    const unsigned m = __ballot_sync(0xffffffffu, crosses(c + 1 + lane));
+    const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+    c += run;
+    if (run < 32) break;
+  }
+  *last = c;
+}
+
+// A block adds the rows of a range of the sorted tokens, in a slice of the
+// columns; a warp takes a part of the range.  Runs inside a warp's part are
+// written at once, those over the edges of parts are joined through shared
+// memory, those over the edges of the range through the workspace by the block
+// that comes last: always in the tokens' order.
 template <typename TG, typename TO, bool kVector>
 __global__ void __launch_bounds__(kSumThreads) SumRunsKernel(SumParams p) {
   using S = Slice<TG, kVector>;
-  constexpr int kCols = S::kCols, kAhead = 4;
-  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
-  if (item >= static_cast<uint64_t>(p.chunks) * p.tiles) return;
-  const uint32_t chunk = static_cast<uint32_t>(item / p.tiles);
-  const S slice(static_cast<uint32_t>(item - static_cast<uint64_t>(chunk) * p.tiles), p.width);
-  const int lane = threadIdx.x & 31;
-  const uint32_t i0 = chunk * kChunkTokens;
-  const int count = static_cast<int>(min(static_cast<uint32_t>(kChunkTokens), p.n - i0));
+  constexpr int kCols = S::kCols;
+  __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
+  __shared__ uint32_t before_key[kSumWarps], first_key[kSumWarps], last_key[kSumWarps], behind_key[kSumWarps];
+  __shared__ uint32_t run_first, run_last, is_last;
+  const uint32_t range = blockIdx.x / p.tiles, tile = blockIdx.x - range * p.tiles;
+  const S slice(tile, p.width);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t i0 = (range * kSumWarps + warp) * p.per_warp;
+  const int count = i0 < p.n ? static_cast<int>(min(p.per_warp, p.n - i0)) : 0;
   const uint32_t key = lane < count ? p.key[i0 + lane] : kNoKey;
   const uint32_t position = lane < count ? p.position[i0 + lane] : 0;
-  const uint32_t before = i0 > 0 ? p.key[i0 - 1] : kNoKey;
-  const uint32_t behind = i0 + count < p.n ? p.key[i0 + count] : kNoKey;
-  const int known = __popc(__ballot_sync(0xffffffffu, key < p.rows));  // those without a row come last
+  const uint32_t before = count > 0 && i0 > 0 ? p.key[i0 - 1] : kNoKey;
+  const uint32_t behind = count > 0 && i0 + count < p.n ? p.key[i0 + count] : kNoKey;
+  const int known = __popc(__ballot_sync(0xffffffffu, key < p.rows));  // tokens without a row come last
   const TG* grad = static_cast<const TG*>(p.grad);
   float sum[kCols];
 #pragma unroll
   for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
-  bool first = true;  // the run that is being added began at the chunk's first token
+  bool first = true;  // the run that is being added began with the part's first token
   for (int j = 0; j < known; j += kAhead) {
-    float a[kAhead][kCols];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (j + u < known) slice.Load(grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j + u)) * p.width, a[u]);
+    typename S::Raw raw[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (j + u >= known) break;
+      const uint32_t at = __shfl_sync(0xffffffffu, position, (j + u) & 31);
+      if (j + u < known) slice.LoadRaw(grad + static_cast<uint64_t>(at) * p.width, &raw[u]);
+    }
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) sum[e] += a[u][e];
-      const uint32_t k = __shfl_sync(0xffffffffu, key, j + u);
-      const uint32_t next = j + u + 1 < count ? __shfl_sync(0xffffffffu, key, (j + u + 1) & 31) : behind;
-      const bool last = j + u + 1 == count;
-      if (k == next && !last) continue;
-      const bool from_before = first && before == k;
-      if (from_before || (last && next == k)) {
-        slice.Store(p.partial + (2 * static_cast<uint64_t>(chunk) + (from_before ? 0 : 1)) * p.width, sum);
-      } else {
-        WriteRow<TO>(p, slice, k, sum);
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u < known) {
+        S::AddRaw(raw[u], sum);
+        const uint32_t k = __shfl_sync(0xffffffffu, key, j + u);
+        const uint32_t next = j + u + 1 < count ? __shfl_sync(0xffffffffu, key, (j + u + 1) & 31) : behind;
+        const bool last = j + u + 1 == count;
+        if (k != next || last) {
+          const bool from_before = first && before == k;
+          if (from_before || k == next) {
+            float* mine = part[warp][from_before ? 0 : 1];
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) mine[e * 32 + lane] = sum[e];
+          } else {
+            WriteRow<TO>(p, slice, k, sum);
+          }
+          first = false;
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+        }
       }
-      first = false;
-#pragma unroll
-      for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
     }
   }
-}
-
-// The runs that go over a chunk's edge: the chunk in which a run begins adds its parts in order.
-template <typename TG, typename TO, bool kVector>
-__global__ void __launch_bounds__(kSumThreads) JoinRunsKernel(SumParams p) {
-  using S = Slice<TG, kVector>;
-  constexpr int kCols = S::kCols;
-  const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
-  if (item >= static_cast<uint64_t>(p.chunks) * p.tiles) return;
-  const uint32_t chunk = static_cast<uint32_t>(item / p.tiles);
-  const uint32_t i0 = chunk * kChunkTokens;
-  if (p.n - i0 <= kChunkTokens) return;
-  const uint32_t k = p.key[i0 + kChunkTokens - 1];
-  if (k >= p.rows || p.key[i0 + kChunkTokens] != k) return;
-  if (p.key[i0] == k && i0 > 0 && p.key[i0 - 1] == k) return;  // it began in an earlier chunk
-  // The last token of the run.
-  uint32_t lo = i0 + kChunkTokens, hi = p.n;  // key[lo] == k, key[hi] != k
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (p.key[mid] == k) lo = mid;
-    else hi = mid;
+  if (lane == 0) {
+    before_key[warp] = before;
+    first_key[warp] = key;
+    behind_key[warp] = behind;
   }
-  const uint32_t end = lo / kChunkTokens;
-  const S slice(static_cast<uint32_t>(item - static_cast<uint64_t>(chunk) * p.tiles), p.width);
-  float sum[kCols];
-  slice.Load(p.partial + (2 * static_cast<uint64_t>(chunk) + 1) * p.width, sum);
-#pragma unroll 4
-  for (uint32_t c = chunk + 1; c <= end; ++c) {
-    float a[kCols];
-    slice.Load(p.partial + 2 * static_cast<uint64_t>(c) * p.width, a);
+  if (lane == (count > 0 ? count - 1 : 0)) last_key[warp] = key;
+  __syncthreads();
+  // Runs over the edges of parts.
+  const bool from_before = first_key[0] < p.rows && before_key[0] == first_key[0];
+  auto join = [&](int w, bool head) {
+    const uint32_t k = head ? first_key[w] : last_key[w];
+    bool on = last_key[w] == k && behind_key[w] == k;
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) sum[e] += a[e];
+    for (int e = 0; e < kCols; ++e) sum[e] = part[w][head ? 0 : 1][e * 32 + lane];
+    while (on && ++w < kSumWarps) {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] += part[w][0][e * 32 + lane];
+      on = last_key[w] == k && behind_key[w] == k;
+    }
+    if (head || on) slice.Store(p.partial + (2 * static_cast<uint64_t>(range) + (head ? 0 : 1)) * p.width, sum);
+    else WriteRow<TO>(p, slice, k, sum);
+  };
+  if (warp == 0 && from_before) join(0, true);
+  const uint32_t k = last_key[warp];
+  if (k < p.rows && behind_key[warp] == k && !(first_key[warp] == k && before_key[warp] == k)) join(warp, false);
+  // Runs over the edges of the range.
+  const uint32_t end = last_key[kSumWarps - 1];
+  const bool to_behind = end < p.rows && behind_key[kSumWarps - 1] == end && !(from_before && first_key[0] == end);
+  if (!from_before && !to_behind) return;
+  __threadfence();
+  for (int side = from_before ? 0 : 1; side < (to_behind ? 2 : 1); ++side) {
+    const uint32_t row = side == 0 ? first_key[0] : end;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t a, b;
+      RangesOfRun(p, row, range, &a, &b);
+      if (lane == 0) {
+        run_first = a;
+        run_last = b;
+        is_last = atomicAdd(p.arrived + static_cast<uint64_t>(a) * p.tiles + tile, 1u) == b - a;
+      }
+    }
+    __syncthreads();
+    if (!is_last) continue;
+    __threadfence();
+    const uint32_t parts = run_last - run_first + 1;
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(parts) * warp / kSumWarps);
+    const uint32_t stop = static_cast<uint32_t>(static_cast<uint64_t>(parts) * (warp + 1) / kSumWarps);
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+#pragma unroll 4
+    for (uint32_t i = begin; i < stop; ++i) {
+      float a[kCols];
+      // The run goes on behind its first range and began before the others.
+      slice.Load(p.partial + (2 * static_cast<uint64_t>(run_first + i) + (i == 0 ? 1 : 0)) * p.width, a);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] += a[e];
+    }
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) part[warp][0][e * 32 + lane] = sum[e];
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < kSumWarps; ++w) {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) sum[e] += part[w][0][e * 32 + lane];
+      }
+      WriteRow<TO>(p, slice, row, sum);
+    }
   }
-  WriteRow<TO>(p, slice, k, sum);
 }
 
 }  // namespace dev
@@ -430,10 +549,23 @@ cudaError_t LaunchEmbedding(const EmbeddingParams& p, cudaStream_t stream) {
   });
 }
 
+struct SumShape {
+  uint32_t per_warp;
+  uint64_t ranges, most_tiles;  // the tiles are fewest columns wide where a lane has four
+};
+SumShape SumShapeOf(uint64_t n, uint64_t width) {
+  SumShape s;
+  s.per_warp = dev::kMostWarpTokens;
+  const uint64_t per = s.per_warp * dev::kSumWarps;
+  s.ranges = (n + per - 1) / per;
+  s.most_tiles = (width + 127) / 128;
+  return s;
+}
+
 size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
   const SortShape s = ShapeOf(n, rows);
-  const uint64_t chunks = (n + dev::kChunkTokens - 1) / dev::kChunkTokens;
-  return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + 2 * chunks * width * 4;
+  const SumShape sum = SumShapeOf(n, width);
+  return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.most_tiles * 4) + 2 * sum.ranges * width * 4;
 }
 
 cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t stream) {
@@ -467,6 +599,10 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     sort.position[i] = reinterpret_cast<uint32_t*>(take(p.num_tokens * 4));
   }
   sort.counts = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(shape.blocks) << shape.bits << 2));
+  const SumShape part = SumShapeOf(p.num_tokens, p.width);
+  if (part.ranges * part.most_tiles > 0xffffffffull) return cudaErrorInvalidValue;
+  sort.num_zeros = static_cast<uint32_t>(part.ranges * part.most_tiles);
+  sort.zeros = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(sort.num_zeros) * 4));
   const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
   cudaError_t e = AllowSharedMemory(dev::SortTokensKernel, smem);
   if (e != cudaSuccess) return e;
@@ -480,9 +616,11 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   sum.position = sort.position[last];
   sum.n = sort.n;
   sum.rows = sort.rows;
-  sum.chunks = (sort.n + dev::kChunkTokens - 1) / dev::kChunkTokens;
+  sum.per_warp = part.per_warp;
+  sum.ranges = static_cast<uint32_t>(part.ranges);
   sum.grad = p.grad;
   sum.out = p.out;
+  sum.arrived = sort.zeros;
   sum.partial = reinterpret_cast<float*>(work);
   sum.width = p.width;
   sum.scale = static_cast<float>(p.scale);
@@ -495,17 +633,11 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     const bool vector = p.width % kCols == 0 && aligned(p.grad, 16) && aligned(p.out, kCols * sizeof(TO));
     const uint64_t tile = 32 * (vector ? kCols : dev::Slice<TG, false>::kCols);
     const uint64_t tiles = (p.width + tile - 1) / tile;
-    const uint64_t blocks = (sum.chunks * tiles + dev::kSumThreads / 32 - 1) / (dev::kSumThreads / 32);
-    if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+    if (part.ranges * tiles > 0x7fffffffull) return cudaErrorInvalidValue;
     sum.tiles = static_cast<uint32_t>(tiles);
-    const unsigned grid = static_cast<unsigned>(blocks);
-    if (vector) {
-      dev::SumRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-      if (sum.chunks > 1) dev::JoinRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-    } else {
-      dev::SumRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-      if (sum.chunks > 1) dev::JoinRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-    }
+    const unsigned grid = static_cast<unsigned>(part.ranges * tiles);
+    if (vector) dev::SumRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
+    else dev::SumRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
     return cudaGetLastError();
   });
 }
