@@ -48,7 +48,7 @@ class _Embedding(torch.autograd.Function):
         if weight.is_leaf and weight.grad is not None:
             # A gradient without entries costs nothing to add, and takes the way of every other one: autograd makes the
             # stream of `weight.grad` wait for this one, adds other uses of the table and runs the bucket's hook, in that order.
-            none = torch.sparse_coo_tensor(size=weight.shape, dtype=weight.dtype, device=weight.device, check_invariants=False)
+            none = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device, layout=torch.sparse_coo)
             return none, None, None, None, None, None
         # Where nothing is handed on, the stream of the backward call waits at its end.
         done = torch.cuda.current_stream(into.device).record_event()

@@ -209,7 +209,6 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 constexpr int kSumWarps = 8;
 constexpr int kSumThreads = 32 * kSumWarps;
 constexpr int kMostWarpTokens = 16;
-constexpr int kAhead = 8;  // rows in flight per warp
 constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct SumParams {
@@ -229,76 +228,70 @@ struct SumParams {
   int accumulate;
 };
 
-// A warp's slice of a row: kCols columns per lane, adjacent with kVector, else 32 apart.
+// A warp's slice of a row: 256 columns, eight per lane, with kVector in vectors
+// of 16 bytes of the gradient's type, else one by one.
 template <typename TG, bool kVector>
 struct Slice {
-  static constexpr int kCols = kVector ? 16 / static_cast<int>(sizeof(TG)) : 4;
-  struct Raw {
-    uint4 v;
-    TG e[kVector ? 1 : kCols];
-  };
-  uint64_t column;  // the lane's first
+  static constexpr int kCols = 8;
+  static constexpr int kPer = kVector ? 16 / static_cast<int>(sizeof(TG)) : 1;  // adjacent columns
+  static constexpr int kVecs = kCols / kPer;
+  static constexpr int kSlots = sizeof(TG) == 4 ? 4 : 8;  // rows on their way to a warp: 4 KiB
+  static constexpr int kRing = kVector ? kSumWarps * kSlots * kVecs * 512 : 0;
   uint64_t width;
-  __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w) {
-    const int lane = threadIdx.x & 31;
-    column = static_cast<uint64_t>(tile) * (32 * kCols) + (kVector ? lane * kCols : lane);
-  }
-  // With kVector the width is a multiple of kCols: a lane has all of its columns or none.
-  __device__ __forceinline__ void LoadRaw(const TG* row, Raw* r) const {
-    if constexpr (kVector) {
-      if (column < width) r->v = Ld16(row + column);
-      else r->v = make_uint4(0, 0, 0, 0);
-    } else {
+  uint64_t column;  // the lane's first; the others are 32 * kPer apart
+  __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w), column(static_cast<uint64_t>(tile) * (32 * kCols) + (threadIdx.x & 31) * kPer) {}
+  // With kVector the width is a multiple of kPer: a lane has all columns of a vector or none.
+  __device__ __forceinline__ bool Has(int v) const { return column + v * (32 * kPer) < width; }
+
+  // A row into one of the warp's slots, without waiting for it; a lane reads what it has written itself.
+  __device__ __forceinline__ void Fetch(const TG* row, unsigned slot) const {
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) r->e[e] = column + e * 32 < width ? row[column + e * 32] : FromAcc<TG, float>(0.f);
-    }
+    for (int v = 0; v < kVecs; ++v)
+      if (Has(v)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + v * 512), "l"(row + column + v * (32 * kPer)) : "memory");
   }
-  __device__ __forceinline__ static void AddRaw(const Raw& r, float* sum) {
-    if constexpr (kVector) {
-      VecIO<TG>::Add(r.v, sum);
-    } else {
+  __device__ __forceinline__ void AddSlot(const unsigned char* slot, float* sum) const {
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) sum[e] += ToAcc<float, TG>(r.e[e]);
-    }
+    for (int v = 0; v < kVecs; ++v) VecIO<TG>::Add(*reinterpret_cast<const uint4*>(slot + v * 512), sum + v * kPer);
   }
   template <typename T>
   __device__ __forceinline__ void Load(const T* row, float* a) const {
-    if constexpr (kVector) {
-      if (column < width) {
-        LoadValues<T, kCols>(row + column, a);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      if (Has(v)) {
+        if constexpr (kVector) LoadValues<T, kPer>(row + column + v * (32 * kPer), a + v * kPer);
+        else a[v] = ToAcc<float, T>(row[column + v * 32]);
       } else {
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) a[e] = 0.f;
+        for (int e = 0; e < kPer; ++e) a[v * kPer + e] = 0.f;
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kCols; ++e) a[e] = column + e * 32 < width ? ToAcc<float, T>(row[column + e * 32]) : 0.f;
     }
   }
   template <typename T>
   __device__ __forceinline__ void Store(T* row, const float* a) const {
-    if constexpr (kVector) {
-      if (column < width) StoreValues<T, kCols>(row + column, a);
-    } else {
 #pragma unroll
-      for (int e = 0; e < kCols; ++e)
-        if (column + e * 32 < width) row[column + e * 32] = FromAcc<T, float>(a[e]);
+    for (int v = 0; v < kVecs; ++v) {
+      if (Has(v)) {
+        if constexpr (kVector) StoreValues<T, kPer>(row + column + v * (32 * kPer), a + v * kPer);
+        else row[column + v * 32] = FromAcc<T, float>(a[v]);
+      }
     }
   }
   // Added by the memory: nothing to wait for.  Only one warp adds to a row, once.
   __device__ __forceinline__ void Add(float* row, const float* a) const {
-    if constexpr (kVector) {
-      if (column < width) {
 #pragma unroll
-        for (int e = 0; e < kCols; e += 4)
-          asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + column + e), "f"(a[e]), "f"(a[e + 1]), "f"(a[e + 2]),
-                       "f"(a[e + 3])
-                       : "memory");
+    for (int v = 0; v < kVecs; ++v) {
+      if (Has(v)) {
+        float* at = row + column + v * (32 * kPer);
+        if constexpr (kVector) {
+#pragma unroll
+          for (int e = 0; e < kPer; e += 4) {
+            const float* b = a + v * kPer + e;
+            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at + e), "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3]) : "memory");
+          }
+        } else {
+          atomicAdd(at, a[v]);
+        }
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kCols; ++e)
-        if (column + e * 32 < width) atomicAdd(row + column + e * 32, a[e]);
     }
   }
 };
@@ -352,9 +345,10 @@ __device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint
 // memory, those over the edges of the range through the workspace by the block
 // that comes last: always in the tokens' order.
 template <typename TG, typename TO, bool kVector>
-__global__ void __launch_bounds__(kSumThreads) SumRunsKernel(SumParams p) {
+__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(SumParams p) {
   using S = Slice<TG, kVector>;
   constexpr int kCols = S::kCols;
+  extern __shared__ __align__(16) unsigned char ring[];  // S::kRing
   __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
   __shared__ uint32_t before_key[kSumWarps], first_key[kSumWarps], last_key[kSumWarps], behind_key[kSumWarps];
   __shared__ uint32_t run_first, run_last, is_last;
@@ -372,33 +366,68 @@ __global__ void __launch_bounds__(kSumThreads) SumRunsKernel(SumParams p) {
   float sum[kCols];
 #pragma unroll
   for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
-  bool first = true;  // the run that is being added began with the part's first token
-  for (int j = 0; j < known; j += kAhead) {
-    typename S::Raw raw[kAhead];
+  // The tokens that end a run, and whether the first and the last run go over the part's edges.
+  const uint32_t next = __shfl_down_sync(0xffffffffu, key, 1);
+  const unsigned ends = __ballot_sync(0xffffffffu, lane < known && (lane == count - 1 || key != next));
+  const bool began_before = before == __shfl_sync(0xffffffffu, key, 0);
+  const bool goes_on = behind == __shfl_sync(0xffffffffu, key, count > 0 ? count - 1 : 0);
+  bool first = true;
+  // The run that token j ends is complete.
+  auto flush = [&](int j) {
+    const bool head = first && began_before;
+    if (head || (goes_on && j == count - 1)) {
+      float* mine = part[warp][head ? 0 : 1];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t at = __shfl_sync(0xffffffffu, position, (j + u) & 31);
-      if (j + u < known) slice.LoadRaw(grad + static_cast<uint64_t>(at) * p.width, &raw[u]);
+      for (int e = 0; e < kCols; ++e) mine[e * 32 + lane] = sum[e];
+    } else {
+      WriteRow<TO>(p, slice, __shfl_sync(0xffffffffu, key, j), sum);
     }
+    first = false;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (j + u < known) {
-        S::AddRaw(raw[u], sum);
-        const uint32_t k = __shfl_sync(0xffffffffu, key, j + u);
-        const uint32_t next = j + u + 1 < count ? __shfl_sync(0xffffffffu, key, (j + u + 1) & 31) : behind;
-        const bool last = j + u + 1 == count;
-        if (k != next || last) {
-          const bool from_before = first && before == k;
-          if (from_before || k == next) {
-            float* mine = part[warp][from_before ? 0 : 1];
+    for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+  };
+  auto row = [&](int j) { return grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j & 31)) * p.width; };
+  if constexpr (kVector) {
+    constexpr int kSlot = S::kVecs * 512;
+    unsigned char* mine = ring + warp * (S::kSlots * kSlot) + lane * 16;
+    const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
 #pragma unroll
-            for (int e = 0; e < kCols; ++e) mine[e * 32 + lane] = sum[e];
-          } else {
-            WriteRow<TO>(p, slice, k, sum);
-          }
-          first = false;
+    for (int u = 0; u < S::kSlots; ++u) {
+      const TG* r = row(u);
+      if (u < known) slice.Fetch(r, mine_shared + u * kSlot);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    for (int j0 = 0; j0 < known; j0 += S::kSlots) {
 #pragma unroll
-          for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
+      for (int u = 0; u < S::kSlots; ++u) {
+        const int j = j0 + u;
+        if (j < known) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
+          slice.AddSlot(mine + u * kSlot, sum);
+          const TG* r = row(j + S::kSlots);
+          if (j + S::kSlots < known) slice.Fetch(r, mine_shared + u * kSlot);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (ends >> j & 1) flush(j);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    constexpr int kTogether = 4;
+    for (int j0 = 0; j0 < known; j0 += kTogether) {
+      TG v[kTogether][kCols];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const TG* r = row(j0 + u);
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) v[u][e] = j0 + u < known && slice.Has(e) ? r[slice.column + e * 32] : FromAcc<TG, float>(0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        if (j0 + u < known) {
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) sum[e] += ToAcc<float, TG>(v[u][e]);
+          if (ends >> (j0 + u) & 1) flush(j0 + u);
         }
       }
     }
@@ -551,21 +580,21 @@ cudaError_t LaunchEmbedding(const EmbeddingParams& p, cudaStream_t stream) {
 
 struct SumShape {
   uint32_t per_warp;
-  uint64_t ranges, most_tiles;  // the tiles are fewest columns wide where a lane has four
+  uint64_t ranges, tiles;
 };
 SumShape SumShapeOf(uint64_t n, uint64_t width) {
   SumShape s;
   s.per_warp = dev::kMostWarpTokens;
   const uint64_t per = s.per_warp * dev::kSumWarps;
   s.ranges = (n + per - 1) / per;
-  s.most_tiles = (width + 127) / 128;
+  s.tiles = (width + 255) / 256;
   return s;
 }
 
 size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
   const SortShape s = ShapeOf(n, rows);
   const SumShape sum = SumShapeOf(n, width);
-  return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.most_tiles * 4) + 2 * sum.ranges * width * 4;
+  return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.tiles * 4) + 2 * sum.ranges * width * 4;
 }
 
 cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t stream) {
@@ -600,8 +629,8 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   }
   sort.counts = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(shape.blocks) << shape.bits << 2));
   const SumShape part = SumShapeOf(p.num_tokens, p.width);
-  if (part.ranges * part.most_tiles > 0xffffffffull) return cudaErrorInvalidValue;
-  sort.num_zeros = static_cast<uint32_t>(part.ranges * part.most_tiles);
+  if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
+  sort.num_zeros = static_cast<uint32_t>(part.ranges * part.tiles);
   sort.zeros = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(sort.num_zeros) * 4));
   const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
   cudaError_t e = AllowSharedMemory(dev::SortTokensKernel, smem);
@@ -618,6 +647,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   sum.rows = sort.rows;
   sum.per_warp = part.per_warp;
   sum.ranges = static_cast<uint32_t>(part.ranges);
+  sum.tiles = static_cast<uint32_t>(part.tiles);
   sum.grad = p.grad;
   sum.out = p.out;
   sum.arrived = sort.zeros;
@@ -628,17 +658,17 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
     using TG = decltype(tg);
     using TO = decltype(to);
-    constexpr uint64_t kCols = dev::Slice<TG, true>::kCols;
+    constexpr uint64_t kPer = dev::Slice<TG, true>::kPer;
     auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
-    const bool vector = p.width % kCols == 0 && aligned(p.grad, 16) && aligned(p.out, kCols * sizeof(TO));
-    const uint64_t tile = 32 * (vector ? kCols : dev::Slice<TG, false>::kCols);
-    const uint64_t tiles = (p.width + tile - 1) / tile;
-    if (part.ranges * tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-    sum.tiles = static_cast<uint32_t>(tiles);
-    const unsigned grid = static_cast<unsigned>(part.ranges * tiles);
-    if (vector) dev::SumRunsKernel<TG, TO, true><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-    else dev::SumRunsKernel<TG, TO, false><<<grid, dev::kSumThreads, 0, stream>>>(sum);
-    return cudaGetLastError();
+    const bool vector = p.width % kPer == 0 && aligned(p.grad, 16) && aligned(p.out, kPer * sizeof(TO));
+    const unsigned grid = static_cast<unsigned>(part.ranges * part.tiles);
+    auto launch = [&](auto kernel, int ring) {
+      const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
+      if (e != cudaSuccess) return e;
+      kernel<<<grid, dev::kSumThreads, ring, stream>>>(sum);
+      return cudaGetLastError();
+    };
+    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
   });
 }
 
