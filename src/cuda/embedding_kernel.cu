@@ -90,6 +90,17 @@ __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __
 }
 
 // -------------------------------------------------------------------- sort
+// The lanes of the warp with the same `bits` lowest bits of `d`, of those in `lanes`.
+__device__ __forceinline__ unsigned Peers(unsigned lanes, uint32_t d, int bits) {
+  unsigned peers = lanes;
+  for (int b = 0; b < bits; ++b) {
+    const bool set = d >> b & 1;
+    const unsigned with = __ballot_sync(0xffffffffu, set);
+    peers &= set ? with : ~with;
+  }
+  return peers;
+}
+
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMostDigitBits = 10;
@@ -188,13 +199,13 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
       const uint32_t i = i0 + lane;
       const bool valid = i < end;
       const unsigned active = __ballot_sync(0xffffffffu, valid);
+      const uint32_t k = !valid ? 0 : pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
+      const uint32_t at = !valid || pass == 0 ? i : __ldcg(position_in + i);
+      const uint32_t d = (k >> shift) & (bins - 1);
+      const unsigned peers = Peers(active, d, p.bits);
+      const uint32_t place = mine[d] + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
       if (valid) {
-        const uint32_t k = pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
-        const uint32_t at = pass == 0 ? i : __ldcg(position_in + i);
-        const uint32_t d = (k >> shift) & (bins - 1);
-        const unsigned peers = __match_any_sync(active, d);
-        const uint32_t place = mine[d] + __popc(peers & ((1u << lane) - 1));
-        __syncwarp(active);
         if (lane == 31 - __clz(peers)) mine[d] = place + 1;
         __stcg(key_out + place, k);
         __stcg(position_out + place, at);
@@ -202,6 +213,142 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
       __syncwarp();
     }
     if (pass + 1 < p.passes) grid.sync();
+  }
+}
+
+// The same within one thread-block cluster, for lists that fit into its shared
+// memory: a thread holds kItems elements in registers, counts go from block to
+// block through distributed shared memory, elements are placed in the shared
+// memory of the block that has them in the next pass.  The other clusters of the
+// grid clear the table at the same time.
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterBlocks = 8;  // at most
+constexpr int kMostItems = 16;
+
+struct ClearParams {
+  unsigned char* out;
+  uint64_t bytes;
+};
+
+constexpr uint64_t kClearBytes = 128 << 10;  // of a block
+
+// Block `block`'s part, in 32-byte stores.
+__device__ __forceinline__ void Clear(const ClearParams& c, uint64_t block) {
+  const uint64_t head = min(static_cast<uint64_t>((32 - reinterpret_cast<uintptr_t>(c.out) % 32) % 32), c.bytes);
+  const uint64_t quanta = (c.bytes - head) / 32;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint64_t end = min(quanta, (block + 1) * (kClearBytes / 32));
+#pragma unroll 4
+  for (uint64_t q = block * (kClearBytes / 32) + threadIdx.x; q < end; q += kClusterThreads) St32(c.out + head + q * 32, zero, zero);
+  const uint64_t tail = head + quanta * 32;
+  if (block == 0 && threadIdx.x < head) c.out[threadIdx.x] = 0;
+  if (block == 0 && threadIdx.x < c.bytes - tail) c.out[tail + threadIdx.x] = 0;
+}
+
+template <int kItems>
+__global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams p, ClearParams clear) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const uint32_t blocks = cluster.num_blocks();
+  if (blockIdx.x >= blocks) {
+    Clear(clear, blockIdx.x - blocks);
+    return;
+  }
+  constexpr uint32_t kPerBlock = kItems * kClusterThreads;
+  const int bins = 1 << p.bits;
+  uint2* elements = reinterpret_cast<uint2*>(memory);                                       // kPerBlock
+  uint32_t* totals = reinterpret_cast<uint32_t*>(memory + kPerBlock * sizeof(uint2));       // bins
+  uint32_t* bases = totals + bins;                                                          // bins
+  unsigned short* counts = reinterpret_cast<unsigned short*>(bases + bins);                 // kClusterWarps x bins
+  __shared__ uint32_t scan[kClusterWarps];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  unsigned short* mine = counts + warp * bins;
+  for (uint32_t i = blockIdx.x * kClusterThreads + threadIdx.x; i < p.num_zeros; i += blocks * kClusterThreads) p.zeros[i] = 0;
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    uint32_t key[kItems], position[kItems], rank[kItems];
+    const uint32_t first = warp * (32 * kItems) + lane;  // in the block; a warp's elements are adjacent
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t at = first + i * 32, t = blockIdx.x * kPerBlock + at;
+      if (pass == 0) {
+        key[i] = t < p.n ? KeyOf(p, t) : 0;
+        position[i] = t;
+      } else {
+        const uint2 e = elements[at];
+        key[i] = e.x;
+        position[i] = e.y;
+      }
+    }
+    for (int i = threadIdx.x; i < kClusterWarps * bins / 2; i += kClusterThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0;
+    __syncthreads();
+    // A place among the warp's elements of the same digit, in their order.
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const bool valid = blockIdx.x * kPerBlock + first + i * 32 < p.n;
+      const uint32_t d = (key[i] >> shift) & (bins - 1);
+      const unsigned peers = Peers(__ballot_sync(0xffffffffu, valid), d, p.bits);
+      rank[i] = valid ? mine[d] + __popc(peers & ((1u << lane) - 1)) : 0;
+      __syncwarp();
+      if (valid && lane == 31 - __clz(peers)) mine[d] = static_cast<unsigned short>(rank[i] + 1);
+      __syncwarp();
+    }
+    __syncthreads();
+    // Of every digit, what the warps before have and what the block has.
+    if (static_cast<int>(threadIdx.x) < bins) {
+      uint32_t sum = 0;
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const uint32_t c = counts[w * bins + threadIdx.x];
+        counts[w * bins + threadIdx.x] = static_cast<unsigned short>(sum);
+        sum += c;
+      }
+      totals[threadIdx.x] = sum;
+    }
+    cluster.sync();  // the totals are there, and all elements are in registers
+    uint32_t before = 0, all = 0;
+    if (static_cast<int>(threadIdx.x) < bins) {
+#pragma unroll
+      for (int b = 0; b < kClusterBlocks; ++b) {
+        const uint32_t c = b < static_cast<int>(blocks) ? *cluster.map_shared_rank(totals + threadIdx.x, b) : 0;
+        before += b < static_cast<int>(blockIdx.x) ? c : 0;
+        all += c;
+      }
+    }
+    uint32_t inclusive = all;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inclusive, s);
+      if (lane >= s) inclusive += v;
+    }
+    if (lane == 31) scan[warp] = inclusive;
+    __syncthreads();
+    uint32_t smaller = scan[lane];  // kClusterWarps is 32
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, smaller, s);
+      if (lane >= s) smaller += v;
+    }
+    smaller = __shfl_sync(0xffffffffu, smaller, (warp + 31) & 31);
+    if (static_cast<int>(threadIdx.x) < bins) bases[threadIdx.x] = (warp > 0 ? smaller : 0) + inclusive - all + before;
+    __syncthreads();
+    const bool last = pass + 1 == p.passes;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (blockIdx.x * kPerBlock + first + i * 32 < p.n) {
+        const uint32_t d = (key[i] >> shift) & (bins - 1);
+        const uint32_t place = bases[d] + mine[d] + rank[i];
+        if (last) {
+          p.key[0][place] = key[i];
+          p.position[0][place] = position[i];
+        } else {
+          *cluster.map_shared_rank(elements + place % kPerBlock, place / kPerBlock) = make_uint2(key[i], position[i]);
+        }
+      }
+    }
+    // The elements are there; in the last pass, nobody reads this block's totals any more.
+    cluster.sync();
   }
 }
 
@@ -228,15 +375,18 @@ struct SumParams {
   int accumulate;
 };
 
-// A warp's slice of a row: 256 columns, eight per lane, with kVector in vectors
-// of 16 bytes of the gradient's type, else one by one.
-template <typename TG, bool kVector>
+// A warp's slice of a row: 256 columns, eight per lane: with kVector in vectors
+// of at most 16 bytes of either type (a warp's access is one stretch of memory in
+// both), else one by one.
+template <typename TG, typename TO, bool kVector>
 struct Slice {
   static constexpr int kCols = 8;
-  static constexpr int kPer = kVector ? 16 / static_cast<int>(sizeof(TG)) : 1;  // adjacent columns
+  static constexpr int kPer = !kVector ? 1 : sizeof(TG) == 2 && sizeof(TO) == 2 ? 8 : 4;  // adjacent columns
   static constexpr int kVecs = kCols / kPer;
-  static constexpr int kSlots = sizeof(TG) == 4 ? 4 : 8;  // rows on their way to a warp: 4 KiB
-  static constexpr int kRing = kVector ? kSumWarps * kSlots * kVecs * 512 : 0;
+  static constexpr int kVecBytes = kPer * static_cast<int>(sizeof(TG));
+  static constexpr int kSlotBytes = 32 * kCols * static_cast<int>(sizeof(TG));
+  static constexpr int kSlots = 4096 / kSlotBytes;  // rows on their way to a warp
+  static constexpr int kRing = kVector ? kSumWarps * kSlots * kSlotBytes : 0;
   uint64_t width;
   uint64_t column;  // the lane's first; the others are 32 * kPer apart
   __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w), column(static_cast<uint64_t>(tile) * (32 * kCols) + (threadIdx.x & 31) * kPer) {}
@@ -247,11 +397,25 @@ struct Slice {
   __device__ __forceinline__ void Fetch(const TG* row, unsigned slot) const {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
-      if (Has(v)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + v * 512), "l"(row + column + v * (32 * kPer)) : "memory");
+      if (Has(v)) {
+        const TG* from = row + column + v * (32 * kPer);
+        if constexpr (kVecBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + v * 512), "l"(from) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(slot + v * 256), "l"(from) : "memory");
+      }
   }
   __device__ __forceinline__ void AddSlot(const unsigned char* slot, float* sum) const {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) VecIO<TG>::Add(*reinterpret_cast<const uint4*>(slot + v * 512), sum + v * kPer);
+    for (int v = 0; v < kVecs; ++v) {
+      if constexpr (kVecBytes == 16) {
+        VecIO<TG>::Add(*reinterpret_cast<const uint4*>(slot + v * 512), sum + v * kPer);
+      } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(slot + v * 256);
+        float a[8];
+        VecIO<TG>::Load(make_uint4(q.x, q.y, 0, 0), a);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum[v * kPer + e] += a[e];
+      }
+    }
   }
   template <typename T>
   __device__ __forceinline__ void Load(const T* row, float* a) const {
@@ -346,7 +510,7 @@ __device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint
 // that comes last: always in the tokens' order.
 template <typename TG, typename TO, bool kVector>
 __global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(SumParams p) {
-  using S = Slice<TG, kVector>;
+  using S = Slice<TG, TO, kVector>;
   constexpr int kCols = S::kCols;
   extern __shared__ __align__(16) unsigned char ring[];  // S::kRing
   __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
@@ -388,8 +552,8 @@ __global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(Su
   };
   auto row = [&](int j) { return grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j & 31)) * p.width; };
   if constexpr (kVector) {
-    constexpr int kSlot = S::kVecs * 512;
-    unsigned char* mine = ring + warp * (S::kSlots * kSlot) + lane * 16;
+    constexpr int kSlot = S::kSlotBytes;
+    unsigned char* mine = ring + warp * (S::kSlots * kSlot) + lane * S::kVecBytes;
     const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
 #pragma unroll
     for (int u = 0; u < S::kSlots; ++u) {
@@ -551,6 +715,7 @@ cudaError_t WithTypes(int dtype_in, int dtype_out, F f) {
 struct SortShape {
   int passes, bits, blocks;
   uint32_t per_block;
+  int items;  // per thread of a cluster's blocks; 0: the cooperative kernel
 };
 SortShape ShapeOf(uint64_t n, uint64_t rows) {
   SortShape s;
@@ -558,6 +723,16 @@ SortShape ShapeOf(uint64_t n, uint64_t rows) {
   while (all < 32 && (rows >> all) != 0) ++all;
   s.passes = (all + dev::kMostDigitBits - 1) / dev::kMostDigitBits;
   s.bits = (all + s.passes - 1) / s.passes;
+  // In a cluster, as few blocks and elements per thread as hold the list.
+  s.items = 0;
+  if (n <= static_cast<uint64_t>(dev::kClusterBlocks) * dev::kMostItems * dev::kClusterThreads) {
+    s.blocks = 1;
+    s.items = 1;
+    while (s.blocks < dev::kClusterBlocks && static_cast<uint64_t>(s.blocks) * dev::kClusterThreads < n) s.blocks *= 2;
+    while (static_cast<uint64_t>(s.blocks) * s.items * dev::kClusterThreads < n) s.items *= 2;
+    s.per_block = 0;
+    return s;
+  }
   // A block takes at least 2048 tokens: with fewer the blocks' counts cost more than the tokens.
   uint64_t blocks = std::min<uint64_t>(std::max<uint64_t>((n + 2047) / 2048, 1), dev::kMostSortBlocks);
   uint64_t per = (n + blocks - 1) / blocks;
@@ -568,6 +743,30 @@ SortShape ShapeOf(uint64_t n, uint64_t rows) {
 }
 
 size_t Padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+template <int kItems>
+cudaError_t LaunchClusterSort(const dev::SortParams& sort, const SortShape& shape, const dev::ClearParams& clear, cudaStream_t stream) {
+  const size_t bins = static_cast<size_t>(1) << shape.bits;
+  const size_t smem = static_cast<size_t>(kItems) * dev::kClusterThreads * sizeof(uint2) + bins * 8 + bins * dev::kClusterWarps * 2;
+  auto kernel = dev::ClusterSortKernel<kItems>;
+  cudaError_t e = AllowSharedMemory(kernel, smem);
+  if (e != cudaSuccess) return e;
+  const uint64_t parts = (clear.bytes + dev::kClearBytes - 1) / dev::kClearBytes;
+  const uint64_t clusters = (parts + shape.blocks - 1) / shape.blocks;
+  if (clusters >= 0x7fffffffull / shape.blocks) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(shape.blocks * (1 + clusters)));
+  config.blockDim = dim3(dev::kClusterThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(shape.blocks);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, sort, clear);
+}
 
 }  // namespace
 
@@ -601,11 +800,8 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   if (p.rows == 0 || p.width == 0) return cudaSuccess;
   if (p.num_tokens > 0x7fffffffull || p.rows > 0x7ffffffeull) return cudaErrorInvalidValue;
   const size_t size_out = static_cast<DType>(p.dtype_out) == DType::kFloat32 ? 4 : 2;
-  if (!p.accumulate) {
-    const cudaError_t e = cudaMemsetAsync(p.out, 0, p.rows * p.width * size_out, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (p.num_tokens == 0) return cudaSuccess;
+  const dev::ClearParams clear{static_cast<unsigned char*>(p.out), p.accumulate ? 0 : p.rows * p.width * size_out};
+  if (p.num_tokens == 0) return clear.bytes > 0 ? cudaMemsetAsync(clear.out, 0, clear.bytes, stream) : cudaSuccess;
   if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
   const SortShape shape = ShapeOf(p.num_tokens, p.rows);
   char* work = static_cast<char*>(p.work);
@@ -632,15 +828,27 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
   sort.num_zeros = static_cast<uint32_t>(part.ranges * part.tiles);
   sort.zeros = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(sort.num_zeros) * 4));
-  const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
-  cudaError_t e = AllowSharedMemory(dev::SortTokensKernel, smem);
-  if (e != cudaSuccess) return e;
-  void* args[] = {&sort};
-  e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&dev::SortTokensKernel), dim3(static_cast<unsigned>(shape.blocks)), dim3(dev::kSortThreads), args,
-                                  smem, stream);
+  cudaError_t e = cudaSuccess;
+  int last = 0;  // which of the two lists is the sorted one
+  switch (shape.items) {
+    case 1: e = LaunchClusterSort<1>(sort, shape, clear, stream); break;
+    case 2: e = LaunchClusterSort<2>(sort, shape, clear, stream); break;
+    case 4: e = LaunchClusterSort<4>(sort, shape, clear, stream); break;
+    case 8: e = LaunchClusterSort<8>(sort, shape, clear, stream); break;
+    case 16: e = LaunchClusterSort<16>(sort, shape, clear, stream); break;
+    default: {
+      if (clear.bytes > 0) e = cudaMemsetAsync(clear.out, 0, clear.bytes, stream);
+      const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
+      if (e == cudaSuccess) e = AllowSharedMemory(dev::SortTokensKernel, smem);
+      void* args[] = {&sort};
+      if (e == cudaSuccess)
+        e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&dev::SortTokensKernel), dim3(static_cast<unsigned>(shape.blocks)), dim3(dev::kSortThreads),
+                                        args, smem, stream);
+      last = (shape.passes - 1) & 1;
+    }
+  }
   if (e != cudaSuccess) return e;
   dev::SumParams sum{};
-  const int last = (shape.passes - 1) & 1;
   sum.key = sort.key[last];
   sum.position = sort.position[last];
   sum.n = sort.n;
@@ -658,9 +866,9 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
     using TG = decltype(tg);
     using TO = decltype(to);
-    constexpr uint64_t kPer = dev::Slice<TG, true>::kPer;
+    constexpr uint64_t kPer = dev::Slice<TG, TO, true>::kPer;
     auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
-    const bool vector = p.width % kPer == 0 && aligned(p.grad, 16) && aligned(p.out, kPer * sizeof(TO));
+    const bool vector = p.width % kPer == 0 && aligned(p.grad, kPer * sizeof(TG)) && aligned(p.out, kPer * sizeof(TO));
     const unsigned grid = static_cast<unsigned>(part.ranges * part.tiles);
     auto launch = [&](auto kernel, int ring) {
       const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
@@ -668,7 +876,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
       kernel<<<grid, dev::kSumThreads, ring, stream>>>(sum);
       return cudaGetLastError();
     };
-    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
+    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
   });
 }
 
