@@ -89,6 +89,10 @@ __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __
   else *o = FromAcc<TO, float>(a[0]);
 }
 
+// The kernel behind may be set up while this one runs; it waits before it reads.
+__device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // -------------------------------------------------------------------- sort
 // The lanes of the warp with the same `bits` lowest bits of `d`, of those in `lanes`.
 __device__ __forceinline__ unsigned Peers(unsigned lanes, uint32_t d, int bits) {
@@ -105,6 +109,7 @@ constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMostDigitBits = 10;
 constexpr int kMostSortBlocks = 64;
+constexpr int kBatch = 4;  // elements of a thread that are loaded together
 
 struct SortParams {
   const void* tokens;
@@ -131,7 +136,8 @@ __device__ __forceinline__ uint32_t KeyOf(const SortParams& p, uint32_t t) {
 // A warp places 32 elements at a time in their order, so every pass is stable.
 __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
   extern __shared__ uint32_t warp_counts[];  // kSortWarps x bins
-  __shared__ uint32_t scan[kSortWarps];
+  LetNextStart();
+  __shared__ uint32_t scan[kSortWarps], bases[1 << kMostDigitBits];
   const cooperative_groups::grid_group grid = cooperative_groups::this_grid();
   const int bins = 1 << p.bits;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
@@ -148,17 +154,26 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
     const int shift = pass * p.bits;
     for (int i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads) warp_counts[i] = 0;
     __syncthreads();
-    for (uint32_t i = begin + lane; i < end; i += 32) {
-      const uint32_t k = pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
-      atomicAdd(&mine[(k >> shift) & (bins - 1)], 1u);
+    for (uint32_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t i = i0 + u * 32 + lane;
+        k[u] = i >= end ? 0 : pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i0 + u * 32 + lane < end) atomicAdd(&mine[(k[u] >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortThreads) {
-      uint32_t sum = 0;
+      uint32_t sum = 0, c[kSortWarps];
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) c[w] = warp_counts[w * bins + d];
+#pragma unroll
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = warp_counts[w * bins + d];
         warp_counts[w * bins + d] = sum;
-        sum += c;
+        sum += c[w];
       }
       __stcg(p.counts + static_cast<size_t>(blockIdx.x) * bins + d, sum);
     }
@@ -169,6 +184,7 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
       const int d = d0 + threadIdx.x;
       uint32_t total = 0, before = 0;
       if (d < bins) {
+#pragma unroll 32
         for (uint32_t g = 0; g < gridDim.x; ++g) {
           const uint32_t c = __ldcg(p.counts + static_cast<size_t>(g) * bins + d);
           before += g < blockIdx.x ? c : 0;
@@ -190,27 +206,33 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
       }
       carried += all;
       if (d < bins) {
-        const uint32_t place = base + inclusive - total + before;
-        for (int w = 0; w < kSortWarps; ++w) warp_counts[w * bins + d] += place;
+        bases[d] = base + inclusive - total + before;
       }
       __syncthreads();
     }
-    for (uint32_t i0 = begin; i0 < end; i0 += 32) {
-      const uint32_t i = i0 + lane;
-      const bool valid = i < end;
-      const unsigned active = __ballot_sync(0xffffffffu, valid);
-      const uint32_t k = !valid ? 0 : pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
-      const uint32_t at = !valid || pass == 0 ? i : __ldcg(position_in + i);
-      const uint32_t d = (k >> shift) & (bins - 1);
-      const unsigned peers = Peers(active, d, p.bits);
-      const uint32_t place = mine[d] + __popc(peers & ((1u << lane) - 1));
-      __syncwarp();
-      if (valid) {
-        if (lane == 31 - __clz(peers)) mine[d] = place + 1;
-        __stcg(key_out + place, k);
-        __stcg(position_out + place, at);
+    for (uint32_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+      uint32_t k[kBatch], at[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t i = i0 + u * 32 + lane;
+        k[u] = i >= end ? 0 : pass == 0 ? KeyOf(p, i) : __ldcg(key_in + i);
+        at[u] = i >= end || pass == 0 ? i : __ldcg(position_in + i);
       }
-      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const bool valid = i0 + u * 32 + lane < end;
+        const uint32_t d = (k[u] >> shift) & (bins - 1);
+        const unsigned peers = Peers(__ballot_sync(0xffffffffu, valid), d, p.bits);
+        const uint32_t rank = mine[d] + __popc(peers & ((1u << lane) - 1));
+        const uint32_t place = bases[d] + rank;
+        __syncwarp();
+        if (valid) {
+          if (lane == 31 - __clz(peers)) mine[d] = rank + 1;
+          __stcg(key_out + place, k[u]);
+          __stcg(position_out + place, at[u]);
+        }
+        __syncwarp();
+      }
     }
     if (pass + 1 < p.passes) grid.sync();
   }
@@ -224,7 +246,7 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterBlocks = 8;  // at most
-constexpr int kMostItems = 16;
+constexpr int kMostItems = 4;
 
 struct ClearParams {
   unsigned char* out;
@@ -251,6 +273,7 @@ __global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams 
   extern __shared__ __align__(16) unsigned char memory[];
   const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const uint32_t blocks = cluster.num_blocks();
+  LetNextStart();
   if (blockIdx.x >= blocks) {
     Clear(clear, blockIdx.x - blocks);
     return;
@@ -297,12 +320,13 @@ __global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams 
     __syncthreads();
     // Of every digit, what the warps before have and what the block has.
     if (static_cast<int>(threadIdx.x) < bins) {
-      uint32_t sum = 0;
+      uint32_t sum = 0, c[kClusterWarps];
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) c[w] = counts[w * bins + threadIdx.x];
 #pragma unroll
       for (int w = 0; w < kClusterWarps; ++w) {
-        const uint32_t c = counts[w * bins + threadIdx.x];
         counts[w * bins + threadIdx.x] = static_cast<unsigned short>(sum);
-        sum += c;
+        sum += c[w];
       }
       totals[threadIdx.x] = sum;
     }
@@ -333,22 +357,24 @@ __global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams 
     smaller = __shfl_sync(0xffffffffu, smaller, (warp + 31) & 31);
     if (static_cast<int>(threadIdx.x) < bins) bases[threadIdx.x] = (warp > 0 ? smaller : 0) + inclusive - all + before;
     __syncthreads();
-    const bool last = pass + 1 == p.passes;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       if (blockIdx.x * kPerBlock + first + i * 32 < p.n) {
         const uint32_t d = (key[i] >> shift) & (bins - 1);
         const uint32_t place = bases[d] + mine[d] + rank[i];
-        if (last) {
-          p.key[0][place] = key[i];
-          p.position[0][place] = position[i];
-        } else {
-          *cluster.map_shared_rank(elements + place % kPerBlock, place / kPerBlock) = make_uint2(key[i], position[i]);
-        }
+        *cluster.map_shared_rank(elements + place % kPerBlock, place / kPerBlock) = make_uint2(key[i], position[i]);
       }
     }
-    // The elements are there; in the last pass, nobody reads this block's totals any more.
-    cluster.sync();
+    cluster.sync();  // the elements are there, and nobody reads this block's totals any more
+  }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const uint32_t at = i * kClusterThreads + threadIdx.x, place = blockIdx.x * kPerBlock + at;
+    if (place < p.n) {
+      const uint2 e = elements[at];
+      p.key[0][place] = e.x;
+      p.position[0][place] = e.y;
+    }
   }
 }
 
@@ -507,16 +533,14 @@ __device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint
 // columns; a warp takes a part of the range.  Runs inside a warp's part are
 // written at once, those over the edges of parts are joined through shared
 // memory, those over the edges of the range through the workspace by the block
-// that comes last: always in the tokens' order.
+// that comes last: always in the tokens' order.  `ring`: S::kRing bytes.
 template <typename TG, typename TO, bool kVector>
-__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(SumParams p) {
+__device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uint32_t tile, unsigned char* ring) {
   using S = Slice<TG, TO, kVector>;
   constexpr int kCols = S::kCols;
-  extern __shared__ __align__(16) unsigned char ring[];  // S::kRing
   __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
   __shared__ uint32_t before_key[kSumWarps], first_key[kSumWarps], last_key[kSumWarps], behind_key[kSumWarps];
   __shared__ uint32_t run_first, run_last, is_last;
-  const uint32_t range = blockIdx.x / p.tiles, tile = blockIdx.x - range * p.tiles;
   const S slice(tile, p.width);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t i0 = (range * kSumWarps + warp) * p.per_warp;
@@ -667,6 +691,79 @@ __global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(Su
   }
 }
 
+template <typename TG, typename TO, bool kVector>
+__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(SumParams p) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  WaitForPrevious();
+  const uint32_t range = blockIdx.x / p.tiles;
+  SumRange<TG, TO, kVector>(p, range, blockIdx.x - range * p.tiles, ring);
+}
+
+// Few tokens: every block sorts them all, by counting for each how many come
+// before it, and adds in its slice of the columns.  The blocks behind clear rows
+// that no token names.
+constexpr uint32_t kSmallTokens = kSumThreads;
+constexpr uint32_t kClearRows = 8192;  // of a block, at most
+
+struct SmallParams {
+  SumParams sum;  // key and position are the block's own
+  const void* tokens;
+  int tokens_are_64;
+  int64_t padding;
+  uint32_t clear_rows;  // of a block
+};
+
+template <typename TG, typename TO, bool kVector>
+__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) FewTokensKernel(SmallParams p) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ __align__(16) uint32_t keys[kSmallTokens], sorted[kSmallTokens], positions[kSmallTokens], named[kClearRows / 32];
+  const uint32_t t = threadIdx.x, n = p.sum.n;
+  SortParams of{};
+  of.tokens = p.tokens;
+  of.tokens_are_64 = p.tokens_are_64;
+  of.rows = p.sum.rows;
+  of.padding = p.padding;
+  const uint32_t key = t < n ? KeyOf(of, t) : kNoKey;
+  if (blockIdx.x < p.sum.tiles) {
+    keys[t] = key;
+    __syncthreads();
+    uint32_t rank = 0;
+    const uint4* four = reinterpret_cast<const uint4*>(keys);
+    for (uint32_t j = 0; j < n; j += 4) {
+      const uint4 k = four[j / 4];
+      rank += (k.x < key + (j < t)) + (k.y < key + (j + 1 < t)) + (k.z < key + (j + 2 < t)) + (k.w < key + (j + 3 < t));
+    }
+    if (t < n) {
+      sorted[rank] = key;
+      positions[rank] = t;
+    }
+    __syncthreads();
+    SumParams sum = p.sum;
+    sum.key = sorted;
+    sum.position = positions;
+    SumRange<TG, TO, kVector>(sum, 0, blockIdx.x, ring);
+    return;
+  }
+  const uint32_t first = (blockIdx.x - p.sum.tiles) * p.clear_rows, rows = min(p.clear_rows, p.sum.rows - first);
+  for (uint32_t i = t; i < kClearRows / 32; i += kSumThreads) named[i] = 0;
+  __syncthreads();
+  if (key >= first && key - first < rows) atomicOr(&named[(key - first) / 32], 1u << (key - first) % 32);
+  __syncthreads();
+  // Stores of 16 bytes where a row is made of them.
+  constexpr uint32_t kPer = kVector ? 16 / sizeof(TO) : 1;
+  const uint32_t width = static_cast<uint32_t>(p.sum.width);
+  TO* out = static_cast<TO*>(p.sum.out) + static_cast<uint64_t>(first) * width;
+  const bool wide = kVector && width % kPer == 0 && reinterpret_cast<uintptr_t>(p.sum.out) % 16 == 0;
+  const uint32_t per_row = wide ? width / kPer : width;
+  const uint64_t units = static_cast<uint64_t>(rows) * per_row;
+  for (uint64_t u = t; u < units; u += kSumThreads) {
+    const uint32_t row = static_cast<uint32_t>(u / per_row);
+    if (named[row / 32] >> row % 32 & 1) continue;
+    if (wide) St16(out + u * kPer, make_uint4(0, 0, 0, 0));
+    else out[u] = FromAcc<TO, float>(0.f);
+  }
+}
+
 }  // namespace dev
 
 namespace {
@@ -783,26 +880,22 @@ struct SumShape {
 };
 SumShape SumShapeOf(uint64_t n, uint64_t width) {
   SumShape s;
-  s.per_warp = dev::kMostWarpTokens;
-  const uint64_t per = s.per_warp * dev::kSumWarps;
+  s.per_warp = n > dev::kSmallTokens ? dev::kMostWarpTokens : static_cast<uint32_t>((n + dev::kSumWarps - 1) / dev::kSumWarps);
+  const uint64_t per = std::max<uint64_t>(s.per_warp * dev::kSumWarps, 1);
   s.ranges = (n + per - 1) / per;
   s.tiles = (width + 255) / 256;
   return s;
 }
 
 size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
+  if (n <= dev::kSmallTokens) return 0;
   const SortShape s = ShapeOf(n, rows);
   const SumShape sum = SumShapeOf(n, width);
   return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.tiles * 4) + 2 * sum.ranges * width * 4;
 }
 
-cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t stream) {
-  if (p.rows == 0 || p.width == 0) return cudaSuccess;
-  if (p.num_tokens > 0x7fffffffull || p.rows > 0x7ffffffeull) return cudaErrorInvalidValue;
-  const size_t size_out = static_cast<DType>(p.dtype_out) == DType::kFloat32 ? 4 : 2;
-  const dev::ClearParams clear{static_cast<unsigned char*>(p.out), p.accumulate ? 0 : p.rows * p.width * size_out};
-  if (p.num_tokens == 0) return clear.bytes > 0 ? cudaMemsetAsync(clear.out, 0, clear.bytes, stream) : cudaSuccess;
-  if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
+// Sorts the tokens and clears the table; `sum` gets what lies in the workspace.
+static cudaError_t LaunchSort(const EmbeddingGradParams& p, const dev::ClearParams& clear, dev::SumParams* sum, cudaStream_t stream) {
   const SortShape shape = ShapeOf(p.num_tokens, p.rows);
   char* work = static_cast<char*>(p.work);
   auto take = [&](size_t bytes) {
@@ -813,8 +906,8 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   dev::SortParams sort{};
   sort.tokens = p.tokens;
   sort.tokens_are_64 = p.tokens_are_64;
-  sort.n = static_cast<uint32_t>(p.num_tokens);
-  sort.rows = static_cast<uint32_t>(p.rows);
+  sort.n = sum->n;
+  sort.rows = sum->rows;
   sort.padding = p.padding;
   sort.per_block = shape.per_block;
   sort.passes = shape.passes;
@@ -824,9 +917,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     sort.position[i] = reinterpret_cast<uint32_t*>(take(p.num_tokens * 4));
   }
   sort.counts = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(shape.blocks) << shape.bits << 2));
-  const SumShape part = SumShapeOf(p.num_tokens, p.width);
-  if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-  sort.num_zeros = static_cast<uint32_t>(part.ranges * part.tiles);
+  sort.num_zeros = sum->ranges * sum->tiles;
   sort.zeros = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(sort.num_zeros) * 4));
   cudaError_t e = cudaSuccess;
   int last = 0;  // which of the two lists is the sorted one
@@ -834,8 +925,6 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     case 1: e = LaunchClusterSort<1>(sort, shape, clear, stream); break;
     case 2: e = LaunchClusterSort<2>(sort, shape, clear, stream); break;
     case 4: e = LaunchClusterSort<4>(sort, shape, clear, stream); break;
-    case 8: e = LaunchClusterSort<8>(sort, shape, clear, stream); break;
-    case 16: e = LaunchClusterSort<16>(sort, shape, clear, stream); break;
     default: {
       if (clear.bytes > 0) e = cudaMemsetAsync(clear.out, 0, clear.bytes, stream);
       const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
@@ -847,22 +936,38 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
       last = (shape.passes - 1) & 1;
     }
   }
-  if (e != cudaSuccess) return e;
+  sum->key = sort.key[last];
+  sum->position = sort.position[last];
+  sum->arrived = sort.zeros;
+  sum->partial = reinterpret_cast<float*>(work);
+  return e;
+}
+
+cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t stream) {
+  if (p.rows == 0 || p.width == 0) return cudaSuccess;
+  if (p.num_tokens > 0x7fffffffull || p.rows > 0x7ffffffeull) return cudaErrorInvalidValue;
+  const size_t size_out = static_cast<DType>(p.dtype_out) == DType::kFloat32 ? 4 : 2;
+  const bool few = p.num_tokens > 0 && p.num_tokens <= dev::kSmallTokens;
+  const dev::ClearParams clear{static_cast<unsigned char*>(p.out), p.accumulate ? 0 : p.rows * p.width * size_out};
+  if (p.num_tokens == 0) return clear.bytes > 0 ? cudaMemsetAsync(clear.out, 0, clear.bytes, stream) : cudaSuccess;
+  if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
+  const SumShape part = SumShapeOf(p.num_tokens, p.width);
+  if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
   dev::SumParams sum{};
-  sum.key = sort.key[last];
-  sum.position = sort.position[last];
-  sum.n = sort.n;
-  sum.rows = sort.rows;
+  sum.n = static_cast<uint32_t>(p.num_tokens);
+  sum.rows = static_cast<uint32_t>(p.rows);
   sum.per_warp = part.per_warp;
   sum.ranges = static_cast<uint32_t>(part.ranges);
   sum.tiles = static_cast<uint32_t>(part.tiles);
   sum.grad = p.grad;
   sum.out = p.out;
-  sum.arrived = sort.zeros;
-  sum.partial = reinterpret_cast<float*>(work);
   sum.width = p.width;
   sum.scale = static_cast<float>(p.scale);
   sum.accumulate = p.accumulate ? 1 : 0;
+  if (!few) {
+    const cudaError_t e = LaunchSort(p, clear, &sum, stream);
+    if (e != cudaSuccess) return e;
+  }
   return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
     using TG = decltype(tg);
     using TO = decltype(to);
@@ -870,11 +975,34 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
     const bool vector = p.width % kPer == 0 && aligned(p.grad, kPer * sizeof(TG)) && aligned(p.out, kPer * sizeof(TO));
     const unsigned grid = static_cast<unsigned>(part.ranges * part.tiles);
+    if (few) {
+      dev::SmallParams small{sum, p.tokens, p.tokens_are_64, p.padding, 0};
+      const uint64_t row = p.width * sizeof(TO);
+      small.clear_rows = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(dev::kClearBytes / row, 1), dev::kClearRows));
+      const uint64_t blocks = part.tiles + (p.accumulate ? 0 : (p.rows + small.clear_rows - 1) / small.clear_rows);
+      if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
+      auto launch = [&](auto kernel, int ring) {
+        const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
+        if (e != cudaSuccess) return e;
+        kernel<<<static_cast<unsigned>(blocks), dev::kSumThreads, ring, stream>>>(small);
+        return cudaGetLastError();
+      };
+      return vector ? launch(dev::FewTokensKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::FewTokensKernel<TG, TO, false>, 0);
+    }
     auto launch = [&](auto kernel, int ring) {
       const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
       if (e != cudaSuccess) return e;
-      kernel<<<grid, dev::kSumThreads, ring, stream>>>(sum);
-      return cudaGetLastError();
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(grid);
+      config.blockDim = dim3(dev::kSumThreads);
+      config.dynamicSmemBytes = static_cast<size_t>(ring);
+      config.stream = stream;
+      cudaLaunchAttribute attribute;
+      attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attribute.val.programmaticStreamSerializationAllowed = 1;
+      config.attrs = &attribute;
+      config.numAttrs = 1;
+      return cudaLaunchKernelEx(&config, kernel, sum);
     };
     return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
   });
