@@ -266,11 +266,13 @@ __global__ void __launch_bounds__(kNormThreads) ClipKernel(const __grid_constant
   const double norm = FinishNorm<P>(f, shared);
   double coefficient = f.max_norm / (norm + kClipEps);
   if (coefficient >= 1.0) coefficient = 1.0;  // a NaN stays
-  uint32_t c = RangeBegin(list.chunks, blockIdx.x);
-  const uint32_t end = RangeBegin(list.chunks, blockIdx.x + 1);
-  uint32_t k = c < end ? SpanOf(list, c) : 0;
-  for (; c < end; ++c) {
-    while (k + 1 < list.count && list.span[k + 1].first_chunk <= c) ++k;
+  // From the range's end: what was read last for the norm is still in L2.
+  const uint32_t begin = RangeBegin(list.chunks, blockIdx.x);
+  uint32_t c = RangeBegin(list.chunks, blockIdx.x + 1);
+  uint32_t k = c > begin ? SpanOf(list, c - 1) : 0;
+  while (c > begin) {
+    --c;
+    while (list.span[k].first_chunk > c) --k;
     const Span& s = list.span[k];
     const uint32_t i = c - s.first_chunk;
     // Times one in place: nothing to write.
