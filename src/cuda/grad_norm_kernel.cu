@@ -13,6 +13,8 @@
 // 2^-30, infinities, NaN) the load's squares are taken again in double, so that
 // no norm overflows or vanishes which fp32 can hold.  The partial sums are added
 // in a fixed order: the result does not depend on the order of execution.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -24,6 +26,7 @@ namespace ibcomm {
 namespace dev {
 
 constexpr int kNormThreads = 256;
+constexpr int kBlocksPerSm = 6;
 constexpr int kChunkBytes = 16384;  // of input: two loads per thread
 constexpr double kClipEps = 1e-6;
 
@@ -40,6 +43,7 @@ template <int kMost>
 struct SpanList {
   uint32_t count;
   uint32_t chunks;
+  int in_place;  // every output is its input
   Span span[kMost];
 };
 
@@ -165,25 +169,37 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
   TO* out = reinterpret_cast<TO*>(s.out);
   const A c = static_cast<A>(coefficient);
   const uint64_t base = chunk * kElems;
-  if (s.vector_out) {
-#pragma unroll 2
+  constexpr bool kWhole = sizeof(TI) * kN == 32;
+  struct Raw {
+    uint4 v[kWhole ? 2 : 1];
+  };
+  auto load = [&](uint64_t i, Raw* r) {
+    if constexpr (kWhole) Ld32(in + i, &r->v[0], &r->v[1]);
+    else r->v[0] = Ld16(in + i);
+  };
+  auto store = [&](uint64_t i, const Raw& r) {
+    A a[kN];
+    AO o[kN];
+    VecIO<TI>::Load(r.v[0], a);
+    if constexpr (kWhole) VecIO<TI>::Load(r.v[1], a + VecIO<TI>::kN);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) o[e] = static_cast<AO>(a[e] * c);
+    if constexpr (sizeof(TO) * kN == 32) St32(out + i, VecIO<TO>::Store(o), VecIO<TO>::Store(o + VecIO<TO>::kN));
+    else St16(out + i, VecIO<TO>::Store(o));
+  };
+  if (s.vector_out && base >= s.begin && base + kElems <= s.end) {
+    Raw r[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) load(base + (threadIdx.x + u * kNormThreads) * kN, &r[u]);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) store(base + (threadIdx.x + u * kNormThreads) * kN, r[u]);
+  } else if (s.vector_out) {
     for (int u = 0; u < kLoads; ++u) {
       const uint64_t i = base + (threadIdx.x + u * kNormThreads) * kN;
       if (i >= s.begin && i + kN <= s.end) {
-        A a[kN];
-        AO o[kN];
-        if constexpr (sizeof(TI) * kN == 32) {
-          uint4 lo, hi;
-          Ld32(in + i, &lo, &hi);
-          VecIO<TI>::Load(lo, a);
-          VecIO<TI>::Load(hi, a + VecIO<TI>::kN);
-        } else {
-          VecIO<TI>::Load(Ld16(in + i), a);
-        }
-#pragma unroll
-        for (int e = 0; e < kN; ++e) o[e] = static_cast<AO>(a[e] * c);
-        if constexpr (sizeof(TO) * kN == 32) St32(out + i, VecIO<TO>::Store(o), VecIO<TO>::Store(o + VecIO<TO>::kN));
-        else St16(out + i, VecIO<TO>::Store(o));
+        Raw r;
+        load(i, &r);
+        store(i, r);
       } else {
 #pragma unroll
         for (int e = 0; e < kN; ++e)
@@ -197,22 +213,11 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
   }
 }
 
-// The block's chunks: a contiguous range.
-__device__ __forceinline__ uint32_t RangeBegin(uint32_t chunks, uint32_t block) {
-  return static_cast<uint32_t>(static_cast<uint64_t>(chunks) * block / gridDim.x);
-}
-
-// partials[block] (+)= the sum of the block's chunks.
-template <int kMost, GradPower P>
-__global__ void __launch_bounds__(kNormThreads) GradSumKernel(const __grid_constant__ SpanList<kMost> list, SumOf<P>* partials, int first) {
-  __shared__ SumOf<P> shared[kNormThreads / 32];
-  uint32_t c = RangeBegin(list.chunks, blockIdx.x);
-  const uint32_t end = RangeBegin(list.chunks, blockIdx.x + 1);
+template <GradPower P, int kMost>
+__device__ __forceinline__ SumOf<P> SumRange(const SpanList<kMost>& list) {
   SumOf<P> sum = 0;
-  uint32_t k = c < end ? SpanOf(list, c) : 0;
-  for (; c < end; ++c) {
-    while (k + 1 < list.count && list.span[k + 1].first_chunk <= c) ++k;
-    const Span& s = list.span[k];
+  for (uint32_t c = blockIdx.x; c < list.chunks; c += gridDim.x) {
+    const Span& s = list.span[SpanOf(list, c)];
     const uint32_t i = c - s.first_chunk;
     switch (static_cast<DType>(s.dtype_in)) {
       case DType::kFloat32: sum = SumChunk<P, float>(s, i, sum); break;
@@ -221,8 +226,34 @@ __global__ void __launch_bounds__(kNormThreads) GradSumKernel(const __grid_const
       default: sum = SumChunk<P, __nv_bfloat16>(s, i, sum); break;
     }
   }
-  sum = BlockJoin(sum, shared);
-  if (threadIdx.x == 0) partials[blockIdx.x] = first ? sum : Join(partials[blockIdx.x], sum);
+  return sum;
+}
+
+template <int kMost>
+__device__ __forceinline__ void ScaleAny(const SpanList<kMost>& list, uint32_t chunk, double coefficient) {
+  const Span& s = list.span[SpanOf(list, chunk)];
+  const uint32_t i = chunk - s.first_chunk;
+  switch (static_cast<DType>(s.dtype_in)) {
+    case DType::kFloat32:
+      if (s.dtype_out == static_cast<int>(DType::kFloat32)) ScaleChunk<float, float>(s, i, coefficient);
+      else if (s.dtype_out == static_cast<int>(DType::kFloat16)) ScaleChunk<float, __half>(s, i, coefficient);
+      else ScaleChunk<float, __nv_bfloat16>(s, i, coefficient);
+      break;
+    case DType::kFloat64: ScaleChunk<double, double>(s, i, coefficient); break;
+    case DType::kFloat16:
+      if (s.dtype_out == static_cast<int>(DType::kFloat16)) ScaleChunk<__half, __half>(s, i, coefficient);
+      else ScaleChunk<__half, float>(s, i, coefficient);
+      break;
+    default:
+      if (s.dtype_out == static_cast<int>(DType::kBFloat16)) ScaleChunk<__nv_bfloat16, __nv_bfloat16>(s, i, coefficient);
+      else ScaleChunk<__nv_bfloat16, float>(s, i, coefficient);
+      break;
+  }
+}
+
+__device__ __forceinline__ double Coefficient(double norm, double max_norm) {
+  const double c = max_norm / (norm + kClipEps);
+  return c >= 1.0 ? 1.0 : c;  // a NaN stays
 }
 
 struct Finish {
@@ -234,13 +265,9 @@ struct Finish {
   double max_norm;
 };
 
-// The sum of all partial sums, in every thread of every block; block 0 writes the results.
+// The norm from the sum of everything; one thread of the grid writes the results.
 template <GradPower P>
-__device__ __forceinline__ double FinishNorm(const Finish& f, SumOf<P>* shared) {
-  const SumOf<P>* sums = reinterpret_cast<const SumOf<P>*>(f.sums);
-  SumOf<P> v = 0;
-  for (int i = threadIdx.x; i < f.num_sums; i += kNormThreads) v = Join(v, sums[i]);
-  v = BlockJoin(v, shared);
+__device__ __forceinline__ double Conclude(const Finish& f, SumOf<P> v) {
   double norm;
   if constexpr (P == GradPower::kTwo) norm = sqrt(v);
   else norm = __longlong_as_double(v);
@@ -254,52 +281,69 @@ __device__ __forceinline__ double FinishNorm(const Finish& f, SumOf<P>* shared) 
   return norm;
 }
 
+// Every block adds the same partial sums in the same order.
+template <GradPower P>
+__device__ __forceinline__ double FinishNorm(const Finish& f, SumOf<P>* shared) {
+  const SumOf<P>* sums = reinterpret_cast<const SumOf<P>*>(f.sums);
+  SumOf<P> v = 0;
+  for (int i = threadIdx.x; i < f.num_sums; i += kNormThreads) v = Join(v, sums[i]);
+  return Conclude<P>(f, BlockJoin(v, shared));
+}
+
+// partials[block] (+)= the sum of the block's chunks.  The kernel behind is set up while the blocks come to their end.
+template <int kMost, GradPower P>
+__global__ void __launch_bounds__(kNormThreads, kBlocksPerSm) GradSumKernel(const __grid_constant__ SpanList<kMost> list, SumOf<P>* partials, int first) {
+  __shared__ SumOf<P> shared[kNormThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const SumOf<P> sum = BlockJoin(SumRange<P>(list), shared);
+  if (threadIdx.x == 0) partials[blockIdx.x] = first ? sum : Join(partials[blockIdx.x], sum);
+}
+
 template <GradPower P>
 __global__ void __launch_bounds__(kNormThreads) FinishNormKernel(Finish f) {
   __shared__ SumOf<P> shared[kNormThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   FinishNorm<P>(f, shared);
 }
 
 template <int kMost, GradPower P>
-__global__ void __launch_bounds__(kNormThreads) ClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f) {
+__global__ void __launch_bounds__(kNormThreads, kBlocksPerSm) ClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f, uint32_t per_block) {
   __shared__ SumOf<P> shared[kNormThreads / 32];
-  const double norm = FinishNorm<P>(f, shared);
-  double coefficient = f.max_norm / (norm + kClipEps);
-  if (coefficient >= 1.0) coefficient = 1.0;  // a NaN stays
-  // From the range's end: what was read last for the norm is still in L2.
-  const uint32_t begin = RangeBegin(list.chunks, blockIdx.x);
-  uint32_t c = RangeBegin(list.chunks, blockIdx.x + 1);
-  uint32_t k = c > begin ? SpanOf(list, c - 1) : 0;
-  while (c > begin) {
-    --c;
-    while (list.span[k].first_chunk > c) --k;
-    const Span& s = list.span[k];
-    const uint32_t i = c - s.first_chunk;
-    // Times one in place: nothing to write.
-    if (coefficient == 1.0 && s.in == s.out && s.dtype_in == s.dtype_out) continue;
-    switch (static_cast<DType>(s.dtype_in)) {
-      case DType::kFloat32:
-        if (s.dtype_out == static_cast<int>(DType::kFloat32)) ScaleChunk<float, float>(s, i, coefficient);
-        else if (s.dtype_out == static_cast<int>(DType::kFloat16)) ScaleChunk<float, __half>(s, i, coefficient);
-        else ScaleChunk<float, __nv_bfloat16>(s, i, coefficient);
-        break;
-      case DType::kFloat64: ScaleChunk<double, double>(s, i, coefficient); break;
-      case DType::kFloat16:
-        if (s.dtype_out == static_cast<int>(DType::kFloat16)) ScaleChunk<__half, __half>(s, i, coefficient);
-        else ScaleChunk<__half, float>(s, i, coefficient);
-        break;
-      default:
-        if (s.dtype_out == static_cast<int>(DType::kBFloat16)) ScaleChunk<__nv_bfloat16, __nv_bfloat16>(s, i, coefficient);
-        else ScaleChunk<__nv_bfloat16, float>(s, i, coefficient);
-        break;
-    }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double c = Coefficient(FinishNorm<P>(f, shared), f.max_norm);
+  // Times one in place: nothing to write.
+  if (c == 1.0 && list.in_place) return;
+  // From the end: what was read last for the norm is still in L2.
+  for (uint32_t u = 0; u < per_block; ++u) {
+    const uint32_t i = blockIdx.x * per_block + u;
+    if (i < list.chunks) ScaleAny(list, list.chunks - 1 - i, c);
   }
+}
+
+// Few chunks: one cluster does everything, with the blocks' sums in its shared memory.
+template <int kMost, GradPower P>
+__global__ void __launch_bounds__(kNormThreads) SmallClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f, int clip) {
+  __shared__ SumOf<P> shared[kNormThreads / 32], mine;
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const SumOf<P> sum = BlockJoin(SumRange<P>(list), shared);
+  if (threadIdx.x == 0) mine = sum;
+  cluster.sync();
+  SumOf<P> v = 0;
+  for (unsigned b = 0; b < gridDim.x; ++b) v = Join(v, *cluster.map_shared_rank(&mine, b));
+  const double norm = Conclude<P>(f, v);
+  const double c = Coefficient(norm, f.max_norm);
+  if (clip && !(c == 1.0 && list.in_place))
+    for (uint32_t i = blockIdx.x; i < list.chunks; i += gridDim.x) ScaleAny(list, i, c);
+  cluster.sync();  // nobody reads this block's sum any more
 }
 
 }  // namespace dev
 
 namespace {
 
+constexpr uint32_t kClusterBlocks = 8, kSmallChunks = 32;
+constexpr uint32_t kMostPerBlock = 4;  // chunks of a block that scales
 constexpr int kMostSpans = 800;  // as many fit into the 32764 bytes of a kernel's parameters
 
 uint32_t SizeOf(int dtype) {
@@ -314,6 +358,7 @@ uint32_t SizeOf(int dtype) {
 template <int kMost>
 void FillList(dev::SpanList<kMost>* list, const GradTensor* tensors, int count, int* next) {
   list->count = 0;
+  list->in_place = 1;
   uint64_t chunks = 0;
   for (; *next < count && list->count < kMost; ++*next) {
     const GradTensor& t = tensors[*next];
@@ -321,7 +366,7 @@ void FillList(dev::SpanList<kMost>* list, const GradTensor* tensors, int count, 
     const uint32_t size = SizeOf(t.dtype_in);
     const uint64_t shift = reinterpret_cast<uintptr_t>(t.in) % 32 / size;
     const uint64_t mine = ((shift + t.n) * size + dev::kChunkBytes - 1) / dev::kChunkBytes;
-    if (chunks + mine > 0xffffffffull) break;
+    if (chunks + mine > 0x7fffffffull) break;
     dev::Span& s = list->span[list->count++];
     s.in = static_cast<const unsigned char*>(t.in) - shift * size;
     s.begin = shift;
@@ -331,6 +376,7 @@ void FillList(dev::SpanList<kMost>* list, const GradTensor* tensors, int count, 
     s.dtype_out = static_cast<uint8_t>(t.dtype_out);
     s.out = nullptr;
     s.vector_out = 0;
+    if (t.out != t.in || t.dtype_out != t.dtype_in) list->in_place = 0;
     if (t.out != nullptr) {
       const uint32_t size_out = SizeOf(t.dtype_out);
       const uint32_t quantum = 32 / std::max(size, size_out) * size_out;
@@ -348,8 +394,30 @@ cudaError_t FullGrid(int* blocks) {
   int device = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  *blocks = std::min(sms * 8, kNormPartials);
+  *blocks = std::min(sms * dev::kBlocksPerSm, kNormPartials);
   return e;
+}
+
+// A launch that is set up while the one before it in the stream comes to its end (the kernel waits before it reads),
+// or as one cluster.
+template <typename... Params, typename... Args>
+cudaError_t Launch(void (*kernel)(Params...), int blocks, bool cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(dev::kNormThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  if (cluster) {
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(blocks);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  } else {
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+  }
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 template <int kMost, GradPower P>
@@ -359,30 +427,42 @@ cudaError_t LaunchTyped(const GradNormParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   dev::SpanList<kMost> list;
   dev::Finish f{p.sums, p.num_sums, p.norm, p.norm_is_double, p.sum, p.max_norm};
+  bool first = true;
   if (p.sums == nullptr) {
     f.sums = p.work;
     f.num_sums = full;
     int next = 0;
-    bool first = true;
     do {
       FillList(&list, p.tensors, p.count, &next);
-      int blocks = full;
-      if (first && next == p.count) blocks = f.num_sums = static_cast<int>(std::min<uint64_t>(full, std::max<uint32_t>(list.chunks, 1)));
-      dev::GradSumKernel<kMost, P><<<blocks, dev::kNormThreads, 0, stream>>>(list, reinterpret_cast<dev::SumOf<P>*>(p.work), first ? 1 : 0);
-      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      const bool all = first && next == p.count;
+      if (all && list.chunks <= kSmallChunks) {
+        const int blocks = static_cast<int>(std::min(std::max(list.chunks, 1u), kClusterBlocks));
+        return Launch(dev::SmallClipKernel<kMost, P>, blocks, true, stream, list, f, p.clip ? 1 : 0);
+      }
+      if (all) f.num_sums = static_cast<int>(std::min<uint64_t>(full, list.chunks));
+      auto* partials = reinterpret_cast<dev::SumOf<P>*>(p.work);
+      // The first launch of a call is an ordinary one: what it reads is written by whatever came before.
+      if (first) dev::GradSumKernel<kMost, P><<<f.num_sums, dev::kNormThreads, 0, stream>>>(list, partials, 1);
+      e = first ? cudaGetLastError() : Launch(dev::GradSumKernel<kMost, P>, f.num_sums, false, stream, list, partials, 0);
+      if (e != cudaSuccess) return e;
       first = false;
     } while (next < p.count);
   }
   if (!p.clip) {
+    if (!first) return Launch(dev::FinishNormKernel<P>, 1, false, stream, f);
     dev::FinishNormKernel<P><<<1, dev::kNormThreads, 0, stream>>>(f);
     return cudaGetLastError();
   }
   int next = 0;
   do {
     FillList(&list, p.tensors, p.count, &next);
-    const int blocks = static_cast<int>(std::min<uint64_t>(full, std::max<uint32_t>(list.chunks, 1)));
-    dev::ClipKernel<kMost, P><<<blocks, dev::kNormThreads, 0, stream>>>(list, f);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const uint32_t per_block = std::min(std::max(list.chunks / static_cast<uint32_t>(2 * full), 1u), kMostPerBlock);
+    const int blocks = static_cast<int>(std::max((list.chunks + per_block - 1) / per_block, 1u));
+    // Behind the sums of the same call, or on its own.
+    if (first) dev::ClipKernel<kMost, P><<<blocks, dev::kNormThreads, 0, stream>>>(list, f, per_block);
+    e = first ? cudaGetLastError() : Launch(dev::ClipKernel<kMost, P>, blocks, false, stream, list, f, per_block);
+    if (e != cudaSuccess) return e;
+    first = true;
   } while (next < p.count);
   return cudaSuccess;
 }
