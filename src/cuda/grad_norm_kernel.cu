@@ -26,7 +26,9 @@ namespace ibcomm {
 namespace dev {
 
 constexpr int kNormThreads = 256;
-constexpr int kBlocksPerSm = 6;
+constexpr int kGroups = 3;       // of kNormThreads, in a block that sums: fewer partial sums for the blocks behind to read
+constexpr int kBlocksPerSm = 2;  // of those; six of the others
+constexpr int kNormCluster = 8;  // blocks of the cluster that takes a short list
 constexpr int kChunkBytes = 16384;  // of input: two loads per thread
 constexpr double kClipEps = 1e-6;
 
@@ -92,17 +94,23 @@ __device__ __forceinline__ SumOf<P> JoinValues(SumOf<P> sum, const A* a) {
   }
 }
 
-// The block's sum, in every thread; the order is that of the threads.
 template <typename S>
-__device__ S BlockJoin(S v, S* shared) {
+__device__ __forceinline__ S WarpJoin(S v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v = Join(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+
+// The block's sum, in every thread; the order is that of the threads.
+template <int kThreads, typename S>
+__device__ S BlockJoin(S v, S* shared) {
+  v = WarpJoin(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
-  for (int w = 0; w < kNormThreads / 32; ++w) v = Join(v, shared[w]);
+  for (int w = 0; w < kThreads / 32; ++w) v = Join(v, shared[w]);
   return v;
 }
 
@@ -124,12 +132,13 @@ __device__ __forceinline__ SumOf<P> SumChunk(const Span& s, uint32_t chunk, SumO
   constexpr int kN = 32 / static_cast<int>(sizeof(T));
   constexpr uint64_t kElems = kChunkBytes / sizeof(T);
   constexpr int kLoads = kChunkBytes / 32 / kNormThreads;
+  const uint32_t thread = threadIdx.x % kNormThreads;
   const T* in = reinterpret_cast<const T*>(s.in);
   const uint64_t base = chunk * kElems;
   if (base >= s.begin && base + kElems <= s.end) {
     uint4 lo[kLoads], hi[kLoads];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) Ld32(in + base + (threadIdx.x + u * kNormThreads) * kN, &lo[u], &hi[u]);
+    for (int u = 0; u < kLoads; ++u) Ld32(in + base + (thread + u * kNormThreads) * kN, &lo[u], &hi[u]);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       A a[kN];
@@ -141,7 +150,7 @@ __device__ __forceinline__ SumOf<P> SumChunk(const Span& s, uint32_t chunk, SumO
   }
 #pragma unroll
   for (int u = 0; u < kLoads; ++u) {
-    const uint64_t i = base + (threadIdx.x + u * kNormThreads) * kN;
+    const uint64_t i = base + (thread + u * kNormThreads) * kN;
     A a[kN];
     if (i >= s.begin && i + kN <= s.end) {
       uint4 lo, hi;
@@ -214,9 +223,9 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
 }
 
 template <GradPower P, int kMost>
-__device__ __forceinline__ SumOf<P> SumRange(const SpanList<kMost>& list) {
+__device__ __forceinline__ SumOf<P> SumRange(const SpanList<kMost>& list, uint32_t first, uint32_t step) {
   SumOf<P> sum = 0;
-  for (uint32_t c = blockIdx.x; c < list.chunks; c += gridDim.x) {
+  for (uint32_t c = first; c < list.chunks; c += step) {
     const Span& s = list.span[SpanOf(list, c)];
     const uint32_t i = c - s.first_chunk;
     switch (static_cast<DType>(s.dtype_in)) {
@@ -281,37 +290,37 @@ __device__ __forceinline__ double Conclude(const Finish& f, SumOf<P> v) {
   return norm;
 }
 
-// Every block adds the same partial sums in the same order.
+// Every warp adds the same partial sums in the same order.
 template <GradPower P>
-__device__ __forceinline__ double FinishNorm(const Finish& f, SumOf<P>* shared) {
+__device__ __forceinline__ double FinishNorm(const Finish& f) {
   const SumOf<P>* sums = reinterpret_cast<const SumOf<P>*>(f.sums);
   SumOf<P> v = 0;
-  for (int i = threadIdx.x; i < f.num_sums; i += kNormThreads) v = Join(v, sums[i]);
-  return Conclude<P>(f, BlockJoin(v, shared));
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < f.num_sums; i += 32) v = Join(v, sums[i]);
+  return Conclude<P>(f, WarpJoin(v));
 }
 
 // partials[block] (+)= the sum of the block's chunks.  The kernel behind is set up while the blocks come to their end.
 template <int kMost, GradPower P>
-__global__ void __launch_bounds__(kNormThreads, kBlocksPerSm) GradSumKernel(const __grid_constant__ SpanList<kMost> list, SumOf<P>* partials, int first) {
-  __shared__ SumOf<P> shared[kNormThreads / 32];
+__global__ void __launch_bounds__(kGroups* kNormThreads, kBlocksPerSm)
+    GradSumKernel(const __grid_constant__ SpanList<kMost> list, SumOf<P>* partials, int first) {
+  __shared__ SumOf<P> shared[kGroups * kNormThreads / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const SumOf<P> sum = BlockJoin(SumRange<P>(list), shared);
+  const SumOf<P> sum = BlockJoin<kGroups * kNormThreads>(SumRange<P>(list, blockIdx.x * kGroups + threadIdx.x / kNormThreads, gridDim.x * kGroups), shared);
   if (threadIdx.x == 0) partials[blockIdx.x] = first ? sum : Join(partials[blockIdx.x], sum);
 }
 
 template <GradPower P>
-__global__ void __launch_bounds__(kNormThreads) FinishNormKernel(Finish f) {
-  __shared__ SumOf<P> shared[kNormThreads / 32];
+__global__ void __launch_bounds__(32) FinishNormKernel(Finish f) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  FinishNorm<P>(f, shared);
+  FinishNorm<P>(f);
 }
 
 template <int kMost, GradPower P>
-__global__ void __launch_bounds__(kNormThreads, kBlocksPerSm) ClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f, uint32_t per_block) {
-  __shared__ SumOf<P> shared[kNormThreads / 32];
+__global__ void __launch_bounds__(kNormThreads, kGroups* kBlocksPerSm) ClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f, uint32_t per_block) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const double c = Coefficient(FinishNorm<P>(f, shared), f.max_norm);
+  const double c = Coefficient(FinishNorm<P>(f), f.max_norm);
   // Times one in place: nothing to write.
   if (c == 1.0 && list.in_place) return;
   // From the end: what was read last for the norm is still in L2.
@@ -326,7 +335,7 @@ template <int kMost, GradPower P>
 __global__ void __launch_bounds__(kNormThreads) SmallClipKernel(const __grid_constant__ SpanList<kMost> list, Finish f, int clip) {
   __shared__ SumOf<P> shared[kNormThreads / 32], mine;
   const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-  const SumOf<P> sum = BlockJoin(SumRange<P>(list), shared);
+  const SumOf<P> sum = BlockJoin<kNormThreads>(SumRange<P>(list, blockIdx.x, gridDim.x), shared);
   if (threadIdx.x == 0) mine = sum;
   cluster.sync();
   SumOf<P> v = 0;
@@ -342,8 +351,8 @@ __global__ void __launch_bounds__(kNormThreads) SmallClipKernel(const __grid_con
 
 namespace {
 
-constexpr uint32_t kClusterBlocks = 8, kSmallChunks = 32;
-constexpr uint32_t kMostPerBlock = 4;  // chunks of a block that scales
+constexpr uint32_t kSmallChunks = 32;   // that one cluster takes
+constexpr uint32_t kMostPerBlock = 8;  // chunks of a block that scales
 constexpr int kMostSpans = 800;  // as many fit into the 32764 bytes of a kernel's parameters
 
 uint32_t SizeOf(int dtype) {
@@ -398,25 +407,26 @@ cudaError_t FullGrid(int* blocks) {
   return e;
 }
 
-// A launch that is set up while the one before it in the stream comes to its end (the kernel waits before it reads),
-// or as one cluster.
+// `early`: the launch is set up while the one before it in the stream comes to its end, and waits before it reads.
 template <typename... Params, typename... Args>
-cudaError_t Launch(void (*kernel)(Params...), int blocks, bool cluster, cudaStream_t stream, const Args&... args) {
+cudaError_t Launch(void (*kernel)(Params...), int blocks, int threads, int cluster, bool early, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(dev::kNormThreads);
+  config.blockDim = dim3(static_cast<unsigned>(threads));
   config.stream = stream;
-  cudaLaunchAttribute attribute;
-  if (cluster) {
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = static_cast<unsigned>(blocks);
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  } else {
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attributes[2];
+  config.attrs = attributes;
+  if (cluster > 1) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = static_cast<unsigned>(cluster);
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
   }
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  if (early) {
+    cudaLaunchAttribute& a = attributes[config.numAttrs++];
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+  }
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
@@ -436,31 +446,25 @@ cudaError_t LaunchTyped(const GradNormParams& p, cudaStream_t stream) {
       FillList(&list, p.tensors, p.count, &next);
       const bool all = first && next == p.count;
       if (all && list.chunks <= kSmallChunks) {
-        const int blocks = static_cast<int>(std::min(std::max(list.chunks, 1u), kClusterBlocks));
-        return Launch(dev::SmallClipKernel<kMost, P>, blocks, true, stream, list, f, p.clip ? 1 : 0);
+        const int blocks = static_cast<int>(std::min(std::max(list.chunks, 1u), static_cast<uint32_t>(dev::kNormCluster)));
+        return Launch(dev::SmallClipKernel<kMost, P>, blocks, dev::kNormThreads, blocks, false, stream, list, f, p.clip ? 1 : 0);
       }
-      if (all) f.num_sums = static_cast<int>(std::min<uint64_t>(full, list.chunks));
-      auto* partials = reinterpret_cast<dev::SumOf<P>*>(p.work);
+      if (all) f.num_sums = static_cast<int>(std::min<uint64_t>(full, (list.chunks + dev::kGroups - 1) / dev::kGroups));
       // The first launch of a call is an ordinary one: what it reads is written by whatever came before.
-      if (first) dev::GradSumKernel<kMost, P><<<f.num_sums, dev::kNormThreads, 0, stream>>>(list, partials, 1);
-      e = first ? cudaGetLastError() : Launch(dev::GradSumKernel<kMost, P>, f.num_sums, false, stream, list, partials, 0);
+      e = Launch(dev::GradSumKernel<kMost, P>, f.num_sums, dev::kGroups * dev::kNormThreads, 1, !first, stream, list, reinterpret_cast<dev::SumOf<P>*>(p.work),
+                 first ? 1 : 0);
       if (e != cudaSuccess) return e;
       first = false;
     } while (next < p.count);
   }
-  if (!p.clip) {
-    if (!first) return Launch(dev::FinishNormKernel<P>, 1, false, stream, f);
-    dev::FinishNormKernel<P><<<1, dev::kNormThreads, 0, stream>>>(f);
-    return cudaGetLastError();
-  }
+  if (!p.clip) return Launch(dev::FinishNormKernel<P>, 1, 32, 1, !first, stream, f);
   int next = 0;
   do {
     FillList(&list, p.tensors, p.count, &next);
-    const uint32_t per_block = std::min(std::max(list.chunks / static_cast<uint32_t>(2 * full), 1u), kMostPerBlock);
+    const uint32_t per_block = std::min(std::max(list.chunks / static_cast<uint32_t>(2 * dev::kGroups * full), 1u), kMostPerBlock);
     const int blocks = static_cast<int>(std::max((list.chunks + per_block - 1) / per_block, 1u));
     // Behind the sums of the same call, or on its own.
-    if (first) dev::ClipKernel<kMost, P><<<blocks, dev::kNormThreads, 0, stream>>>(list, f, per_block);
-    e = first ? cudaGetLastError() : Launch(dev::ClipKernel<kMost, P>, blocks, false, stream, list, f, per_block);
+    e = Launch(dev::ClipKernel<kMost, P>, blocks, dev::kNormThreads, 1, !first, stream, list, f, per_block);
     if (e != cudaSuccess) return e;
     first = true;
   } while (next < p.count);
@@ -476,7 +480,8 @@ cudaError_t LaunchSized(const GradNormParams& p, cudaStream_t stream) {
 
 cudaError_t LaunchGradNorm(const GradNormParams& p, cudaStream_t stream) {
   // A short list has a short block of parameters.
-  return p.count <= 16 ? LaunchSized<16>(p, stream) : LaunchSized<kMostSpans>(p, stream);
+  if (p.count <= 16) return LaunchSized<16>(p, stream);
+  return p.count <= 64 ? LaunchSized<64>(p, stream) : p.count <= 256 ? LaunchSized<256>(p, stream) : LaunchSized<kMostSpans>(p, stream);
 }
 
 }  // namespace ibcomm
