@@ -50,6 +50,7 @@ __device__ __forceinline__ void StoreValues(T* p, const float* a) {
 
 // ------------------------------------------------------------------ lookup
 constexpr int kLookupThreads = 256;
+constexpr int kLookupUnroll = 4;
 
 template <typename TI, typename TO>
 struct LookupQuantum {
@@ -63,30 +64,46 @@ __device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
   else return static_cast<const int*>(tokens)[t];
 }
 
-// A thread per quantum of the output, kN values with kVector, else one.
+// A warp takes kUnroll * 32 quanta of a row (kN values with kVector, else one),
+// all loads before the first store; where a row has fewer than 32, 1 << lanes of
+// the warp's lanes take a row each.  blockIdx.y is the part of the row, so that
+// nothing is divided.
 template <typename TI, typename TO, bool kTokens64, bool kVector>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
-                                                                  uint64_t quanta, uint32_t per_row, uint64_t rows, uint64_t width, float scale) {
+                                                                  uint64_t num_tokens, uint32_t per_row, int lanes, uint64_t rows, uint64_t width, float scale) {
   constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1;
-  const uint64_t q = static_cast<uint64_t>(blockIdx.x) * kLookupThreads + threadIdx.x;
-  if (q >= quanta) return;
-  const uint64_t t = q / per_row;
-  const uint64_t column = (q - t * per_row) * kN;
+  const uint32_t lane = threadIdx.x & 31, group = 1u << lanes;
+  const uint64_t warp = static_cast<uint64_t>(blockIdx.x) * (kLookupThreads / 32) + threadIdx.x / 32;
+  const uint64_t t = (warp << (5 - lanes)) + (lane >> lanes);
+  if (t >= num_tokens) return;
+  const uint32_t first = (blockIdx.y * kLookupUnroll << lanes) + (lane & (group - 1));
   const int64_t id = Token<kTokens64>(tokens, t);
   const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
-  float a[kN];
+  const TI* from = weight + (inside ? static_cast<uint64_t>(id) : 0) * width;
+  TO* to = out + t * width;
+  float a[kLookupUnroll][kN];
 #pragma unroll
-  for (int e = 0; e < kN; ++e) a[e] = 0.f;
-  if (inside) {
-    const TI* p = weight + static_cast<uint64_t>(id) * width + column;
-    if constexpr (kVector) LoadValues<TI, kN>(p, a);
-    else a[0] = ToAcc<float, TI>(*p);
+  for (int u = 0; u < kLookupUnroll; ++u) {
+    const uint32_t q = first + (u << lanes);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) a[e] *= scale;
+    for (int e = 0; e < kN; ++e) a[u][e] = 0.f;
+    if (inside && q < per_row) {
+      if constexpr (kVector) LoadValues<TI, kN>(from + static_cast<uint64_t>(q) * kN, a[u]);
+      else a[u][0] = ToAcc<float, TI>(from[q]);
+    }
   }
-  TO* o = out + t * width + column;
-  if constexpr (kVector) StoreValues<TO, kN>(o, a);
-  else *o = FromAcc<TO, float>(a[0]);
+#pragma unroll
+  for (int u = 0; u < kLookupUnroll; ++u) {
+    const uint32_t q = first + (u << lanes);
+    if (q < per_row) {
+      if (inside) {  // a row that is not there is zero whatever the scale is
+#pragma unroll
+        for (int e = 0; e < kN; ++e) a[u][e] *= scale;
+      }
+      if constexpr (kVector) StoreValues<TO, kN>(to + static_cast<uint64_t>(q) * kN, a[u]);
+      else to[q] = FromAcc<TO, float>(a[u][0]);
+    }
+  }
 }
 
 // The kernel behind may be set up while this one runs; it waits before it reads.
@@ -774,18 +791,19 @@ cudaError_t LaunchLookup(const EmbeddingParams& p, cudaStream_t stream) {
   auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
   const bool vector = p.width % kN == 0 && aligned(p.weight, kN * sizeof(TI)) && aligned(p.out, kN * sizeof(TO));
   const uint64_t per_row = vector ? p.width / kN : p.width;
-  const uint64_t quanta = p.num_tokens * per_row;
-  const uint64_t blocks = (quanta + dev::kLookupThreads - 1) / dev::kLookupThreads;
-  if (blocks > 0x7fffffffull || per_row > 0xffffffffull) return cudaErrorInvalidValue;
+  int lanes = 0;
+  while (lanes < 5 && (1ull << lanes) < per_row) ++lanes;
+  const uint64_t per_block = static_cast<uint64_t>(dev::kLookupThreads) >> lanes;
+  const uint64_t blocks = (p.num_tokens + per_block - 1) / per_block;
+  const uint64_t parts = (per_row + (dev::kLookupUnroll << lanes) - 1) / (dev::kLookupUnroll << lanes);
+  if (blocks > 0x7fffffffull || parts > 65535) return cudaErrorInvalidValue;
   const TI* w = static_cast<const TI*>(p.weight);
   TO* o = static_cast<TO*>(p.out);
-  const unsigned grid = static_cast<unsigned>(blocks);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
   const uint32_t row = static_cast<uint32_t>(per_row);
-  if (vector) {
-    dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, quanta, row, p.rows, p.width, static_cast<float>(p.scale));
-  } else {
-    dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, quanta, row, p.rows, p.width, static_cast<float>(p.scale));
-  }
+  const float scale = static_cast<float>(p.scale);
+  if (vector) dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, lanes, p.rows, p.width, scale);
+  else dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, lanes, p.rows, p.width, scale);
   return cudaGetLastError();
 }
 
