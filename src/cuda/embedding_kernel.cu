@@ -66,17 +66,17 @@ __device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
 
 // A warp takes kUnroll * 32 quanta of a row (kN values with kVector, else one),
 // all loads before the first store; where a row has fewer than 32, 1 << lanes of
-// the warp's lanes take a row each.  blockIdx.y is the part of the row, so that
-// nothing is divided.
+// the warp's lanes take a row each.  The parts of a row are neighbours in the grid.
 template <typename TI, typename TO, bool kTokens64, bool kVector>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
-                                                                  uint64_t num_tokens, uint32_t per_row, int lanes, uint64_t rows, uint64_t width, float scale) {
+                                                                  uint64_t num_tokens, uint32_t per_row, uint32_t parts, int lanes, uint64_t rows, uint64_t width, float scale) {
   constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1;
   const uint32_t lane = threadIdx.x & 31, group = 1u << lanes;
-  const uint64_t warp = static_cast<uint64_t>(blockIdx.x) * (kLookupThreads / 32) + threadIdx.x / 32;
+  const uint32_t block = blockIdx.x / parts, part = blockIdx.x - block * parts;
+  const uint64_t warp = static_cast<uint64_t>(block) * (kLookupThreads / 32) + threadIdx.x / 32;
   const uint64_t t = (warp << (5 - lanes)) + (lane >> lanes);
   if (t >= num_tokens) return;
-  const uint32_t first = (blockIdx.y * kLookupUnroll << lanes) + (lane & (group - 1));
+  const uint32_t first = (part * kLookupUnroll << lanes) + (lane & (group - 1));
   const int64_t id = Token<kTokens64>(tokens, t);
   const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
   const TI* from = weight + (inside ? static_cast<uint64_t>(id) : 0) * width;
@@ -796,14 +796,14 @@ cudaError_t LaunchLookup(const EmbeddingParams& p, cudaStream_t stream) {
   const uint64_t per_block = static_cast<uint64_t>(dev::kLookupThreads) >> lanes;
   const uint64_t blocks = (p.num_tokens + per_block - 1) / per_block;
   const uint64_t parts = (per_row + (dev::kLookupUnroll << lanes) - 1) / (dev::kLookupUnroll << lanes);
-  if (blocks > 0x7fffffffull || parts > 65535) return cudaErrorInvalidValue;
+  if (blocks * parts > 0x7fffffffull) return cudaErrorInvalidValue;
   const TI* w = static_cast<const TI*>(p.weight);
   TO* o = static_cast<TO*>(p.out);
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
+  const unsigned grid = static_cast<unsigned>(blocks * parts);
   const uint32_t row = static_cast<uint32_t>(per_row);
   const float scale = static_cast<float>(p.scale);
-  if (vector) dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, lanes, p.rows, p.width, scale);
-  else dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, lanes, p.rows, p.width, scale);
+  if (vector) dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, static_cast<uint32_t>(parts), lanes, p.rows, p.width, scale);
+  else dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, static_cast<uint32_t>(parts), lanes, p.rows, p.width, scale);
   return cudaGetLastError();
 }
 

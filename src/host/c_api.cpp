@@ -171,9 +171,8 @@ void CheckEmbedding(const void* tokens, int tokens_dtype, size_t num_tokens, siz
   if (t != DType::kInt32 && t != DType::kInt64) IBCOMM_FAIL(NOT_SUPPORTED, "Tokens are int32 or int64, got %s.\n", DTypeName(t));
   for (int d : {table_dtype, values_dtype})
     if (!Floating(d) || CheckDType(d) == DType::kFloat64) IBCOMM_FAIL(NOT_SUPPORTED, "No embedding of %s.\n", DTypeName(CheckDType(d)));
-  // The width: what 65535 blocks of a row of odd length hold.
-  if (num_tokens > 0x7fffffffull || rows > 0x7ffffffeull || width > (1ull << 22))
-    IBCOMM_FAIL(NOT_SUPPORTED, "Tokens and rows are counted in 31 bits, and a row has at most 4194304 columns.\n");
+  if (num_tokens > 0x7fffffffull || rows > 0x7ffffffeull || width > 0x7fffffffull)
+    IBCOMM_FAIL(NOT_SUPPORTED, "Tokens, rows and their width are counted in 31 bits.\n");
   if ((num_tokens > 0 && tokens == nullptr) || (num_tokens > 0 && width > 0 && values == nullptr) || (rows > 0 && width > 0 && table == nullptr))
     IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must have memory.\n");
   if (std::isnan(scale)) IBCOMM_FAIL(INVALID_ARGUMENT, "The scale is not a number.\n");
