@@ -258,43 +258,18 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 // The same within one thread-block cluster, for lists that fit into its shared
 // memory: a thread holds kItems elements in registers, counts go from block to
 // block through distributed shared memory, elements are placed in the shared
-// memory of the block that has them in the next pass.  The other clusters of the
-// grid clear the table at the same time.
+// memory of the block that has them in the next pass.
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterBlocks = 8;  // at most
 constexpr int kMostItems = 4;
 
-struct ClearParams {
-  unsigned char* out;
-  uint64_t bytes;
-};
-
-constexpr uint64_t kClearBytes = 128 << 10;  // of a block
-
-// Block `block`'s part, in 32-byte stores.
-__device__ __forceinline__ void Clear(const ClearParams& c, uint64_t block) {
-  const uint64_t head = min(static_cast<uint64_t>((32 - reinterpret_cast<uintptr_t>(c.out) % 32) % 32), c.bytes);
-  const uint64_t quanta = (c.bytes - head) / 32;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const uint64_t end = min(quanta, (block + 1) * (kClearBytes / 32));
-#pragma unroll 4
-  for (uint64_t q = block * (kClearBytes / 32) + threadIdx.x; q < end; q += kClusterThreads) St32(c.out + head + q * 32, zero, zero);
-  const uint64_t tail = head + quanta * 32;
-  if (block == 0 && threadIdx.x < head) c.out[threadIdx.x] = 0;
-  if (block == 0 && threadIdx.x < c.bytes - tail) c.out[tail + threadIdx.x] = 0;
-}
-
 template <int kItems>
-__global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams p, ClearParams clear) {
+__global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams p) {
   extern __shared__ __align__(16) unsigned char memory[];
   const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   const uint32_t blocks = cluster.num_blocks();
   LetNextStart();
-  if (blockIdx.x >= blocks) {
-    Clear(clear, blockIdx.x - blocks);
-    return;
-  }
   constexpr uint32_t kPerBlock = kItems * kClusterThreads;
   const int bins = 1 << p.bits;
   uint2* elements = reinterpret_cast<uint2*>(memory);                                       // kPerBlock
@@ -393,6 +368,31 @@ __global__ void __launch_bounds__(kClusterThreads) ClusterSortKernel(SortParams 
       p.position[0][place] = e.y;
     }
   }
+}
+
+// ------------------------------------------------------------------- clear
+constexpr int kClearThreads = 256, kClearUnroll = 4;
+constexpr uint64_t kClearBytes = static_cast<uint64_t>(kClearThreads) * kClearUnroll * 32;  // of a block
+
+// out = 0.  It reads nothing, so it runs beside the sort, on the SMs that the sort
+// leaves; its last block waits for the sort, so that whoever waits for this kernel
+// has waited for both.
+__global__ void __launch_bounds__(kClearThreads) ClearKernel(unsigned char* out, uint64_t bytes) {
+  LetNextStart();
+  const uint64_t head = min(static_cast<uint64_t>((32 - reinterpret_cast<uintptr_t>(out) % 32) % 32), bytes);
+  const uint64_t quanta = (bytes - head) / 32;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int u = 0; u < kClearUnroll; ++u) {
+    const uint64_t q = (static_cast<uint64_t>(blockIdx.x) * kClearUnroll + u) * kClearThreads + threadIdx.x;
+    if (q < quanta) St32(out + head + q * 32, zero, zero);
+  }
+  if (blockIdx.x == 0) {
+    const uint64_t tail = head + quanta * 32;
+    if (threadIdx.x < head) out[threadIdx.x] = 0;
+    if (threadIdx.x < bytes - tail) out[tail + threadIdx.x] = 0;
+  }
+  if (blockIdx.x == gridDim.x - 1) WaitForPrevious();
 }
 
 // -------------------------------------------------------------------- sums
@@ -859,18 +859,33 @@ SortShape ShapeOf(uint64_t n, uint64_t rows) {
 
 size_t Padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+constexpr uint64_t kFewClearBytes = 128 << 10;  // of a block that looks for the rows of few tokens
+
+// A launch that may be set up while the one before it in the stream runs.
+template <typename... Params, typename... Args>
+cudaError_t LaunchEarly(void (*kernel)(Params...), unsigned blocks, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 template <int kItems>
-cudaError_t LaunchClusterSort(const dev::SortParams& sort, const SortShape& shape, const dev::ClearParams& clear, cudaStream_t stream) {
+cudaError_t LaunchClusterSort(const dev::SortParams& sort, const SortShape& shape, cudaStream_t stream) {
   const size_t bins = static_cast<size_t>(1) << shape.bits;
   const size_t smem = static_cast<size_t>(kItems) * dev::kClusterThreads * sizeof(uint2) + bins * 8 + bins * dev::kClusterWarps * 2;
   auto kernel = dev::ClusterSortKernel<kItems>;
   cudaError_t e = AllowSharedMemory(kernel, smem);
   if (e != cudaSuccess) return e;
-  const uint64_t parts = (clear.bytes + dev::kClearBytes - 1) / dev::kClearBytes;
-  const uint64_t clusters = (parts + shape.blocks - 1) / shape.blocks;
-  if (clusters >= 0x7fffffffull / shape.blocks) return cudaErrorInvalidValue;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(shape.blocks * (1 + clusters)));
+  config.gridDim = dim3(static_cast<unsigned>(shape.blocks));
   config.blockDim = dim3(dev::kClusterThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
@@ -880,7 +895,7 @@ cudaError_t LaunchClusterSort(const dev::SortParams& sort, const SortShape& shap
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, sort, clear);
+  return cudaLaunchKernelEx(&config, kernel, sort);
 }
 
 }  // namespace
@@ -912,8 +927,8 @@ size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
   return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.tiles * 4) + 2 * sum.ranges * width * 4;
 }
 
-// Sorts the tokens and clears the table; `sum` gets what lies in the workspace.
-static cudaError_t LaunchSort(const EmbeddingGradParams& p, const dev::ClearParams& clear, dev::SumParams* sum, cudaStream_t stream) {
+// Sorts the tokens; `sum` gets what lies in the workspace.
+static cudaError_t LaunchSort(const EmbeddingGradParams& p, dev::SumParams* sum, cudaStream_t stream) {
   const SortShape shape = ShapeOf(p.num_tokens, p.rows);
   char* work = static_cast<char*>(p.work);
   auto take = [&](size_t bytes) {
@@ -940,11 +955,10 @@ static cudaError_t LaunchSort(const EmbeddingGradParams& p, const dev::ClearPara
   cudaError_t e = cudaSuccess;
   int last = 0;  // which of the two lists is the sorted one
   switch (shape.items) {
-    case 1: e = LaunchClusterSort<1>(sort, shape, clear, stream); break;
-    case 2: e = LaunchClusterSort<2>(sort, shape, clear, stream); break;
-    case 4: e = LaunchClusterSort<4>(sort, shape, clear, stream); break;
+    case 1: e = LaunchClusterSort<1>(sort, shape, stream); break;
+    case 2: e = LaunchClusterSort<2>(sort, shape, stream); break;
+    case 4: e = LaunchClusterSort<4>(sort, shape, stream); break;
     default: {
-      if (clear.bytes > 0) e = cudaMemsetAsync(clear.out, 0, clear.bytes, stream);
       const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
       if (e == cudaSuccess) e = AllowSharedMemory(dev::SortTokensKernel, smem);
       void* args[] = {&sort};
@@ -966,8 +980,14 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   if (p.num_tokens > 0x7fffffffull || p.rows > 0x7ffffffeull) return cudaErrorInvalidValue;
   const size_t size_out = static_cast<DType>(p.dtype_out) == DType::kFloat32 ? 4 : 2;
   const bool few = p.num_tokens > 0 && p.num_tokens <= dev::kSmallTokens;
-  const dev::ClearParams clear{static_cast<unsigned char*>(p.out), p.accumulate ? 0 : p.rows * p.width * size_out};
-  if (p.num_tokens == 0) return clear.bytes > 0 ? cudaMemsetAsync(clear.out, 0, clear.bytes, stream) : cudaSuccess;
+  const uint64_t bytes = p.accumulate ? 0 : p.rows * p.width * size_out;
+  const uint64_t clears = (bytes + dev::kClearBytes - 1) / dev::kClearBytes;
+  if (clears > 0x7fffffffull) return cudaErrorInvalidValue;
+  if (p.num_tokens == 0) {
+    if (clears == 0) return cudaSuccess;
+    dev::ClearKernel<<<static_cast<unsigned>(clears), dev::kClearThreads, 0, stream>>>(static_cast<unsigned char*>(p.out), bytes);
+    return cudaGetLastError();
+  }
   if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
   const SumShape part = SumShapeOf(p.num_tokens, p.width);
   if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
@@ -983,7 +1003,9 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   sum.scale = static_cast<float>(p.scale);
   sum.accumulate = p.accumulate ? 1 : 0;
   if (!few) {
-    const cudaError_t e = LaunchSort(p, clear, &sum, stream);
+    cudaError_t e = LaunchSort(p, &sum, stream);
+    if (e == cudaSuccess && clears > 0)
+      e = LaunchEarly(dev::ClearKernel, static_cast<unsigned>(clears), dev::kClearThreads, 0, stream, static_cast<unsigned char*>(p.out), bytes);
     if (e != cudaSuccess) return e;
   }
   return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
@@ -996,7 +1018,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     if (few) {
       dev::SmallParams small{sum, p.tokens, p.tokens_are_64, p.padding, 0};
       const uint64_t row = p.width * sizeof(TO);
-      small.clear_rows = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(dev::kClearBytes / row, 1), dev::kClearRows));
+      small.clear_rows = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(kFewClearBytes / row, 1), dev::kClearRows));
       const uint64_t blocks = part.tiles + (p.accumulate ? 0 : (p.rows + small.clear_rows - 1) / small.clear_rows);
       if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
       auto launch = [&](auto kernel, int ring) {
@@ -1010,17 +1032,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     auto launch = [&](auto kernel, int ring) {
       const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
       if (e != cudaSuccess) return e;
-      cudaLaunchConfig_t config = {};
-      config.gridDim = dim3(grid);
-      config.blockDim = dim3(dev::kSumThreads);
-      config.dynamicSmemBytes = static_cast<size_t>(ring);
-      config.stream = stream;
-      cudaLaunchAttribute attribute;
-      attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attribute.val.programmaticStreamSerializationAllowed = 1;
-      config.attrs = &attribute;
-      config.numAttrs = 1;
-      return cudaLaunchKernelEx(&config, kernel, sum);
+      return LaunchEarly(kernel, grid, dev::kSumThreads, static_cast<size_t>(ring), stream, sum);
     };
     return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
   });
