@@ -10,7 +10,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .._native import IbcommError
@@ -25,36 +24,6 @@ def _check(tokens: torch.Tensor, padding_idx: Optional[int], rows: int) -> int:
     if not 0 <= padding_idx < rows:
         raise IbcommError(_native.INVALID_ARGUMENT, f"padding_idx {padding_idx} is no row of {rows}")
     return int(padding_idx)
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, tokens, scale, padding, out_code, grad_into):
-        ctx.save_for_backward(tokens)
-        ctx.weight = weight
-        ctx.scale, ctx.padding, ctx.grad_into = scale, padding, grad_into
-        return _native.fast().embedding(tokens, weight, out_code, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        (tokens,) = ctx.saved_tensors
-        into, weight = ctx.grad_into, ctx.weight
-        if into is None:
-            into = torch.empty(weight.shape, dtype=weight.dtype, device=grad.device)
-            _native.fast().embedding_grad(tokens, grad.contiguous(), into, ctx.padding, ctx.scale, False)
-            return into, None, None, None, None, None
-        _native.fast().embedding_grad(tokens, grad.contiguous(), into, ctx.padding, ctx.scale, True)
-        if weight.is_leaf and weight.grad is not None:
-            # A gradient without entries costs nothing to add, and takes the way of every other one: autograd makes the
-            # stream of `weight.grad` wait for this one, adds other uses of the table and runs the bucket's hook, in that order.
-            none = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device, layout=torch.sparse_coo)
-            return none, None, None, None, None, None
-        # Where nothing is handed on, the stream of the backward call waits at its end.
-        done = torch.cuda.current_stream(into.device).record_event()
-        torch.autograd.Variable._execution_engine.queue_callback(
-            lambda: torch.cuda.current_stream(into.device).wait_event(done))
-        return None, None, None, None, None, None
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -73,9 +42,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
             raise IbcommError(_native.INVALID_ARGUMENT, "grad_into must be contiguous, of the table's shape and on its GPU")
         if grad_into.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise IbcommError(_native.NOT_SUPPORTED, f"no embedding of {grad_into.dtype}")
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(weight, tokens, float(scale), padding, out_code, grad_into)
-    return _native.fast().embedding(tokens, weight, out_code, float(scale))
+    return _native.fast().embedding(tokens, weight, out_code, float(scale), padding, grad_into)
 
 
 def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, *, out: Optional[torch.Tensor] = None,

@@ -13,12 +13,21 @@
 // them into the Python exceptions torch's own methods raise.
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/Event.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/utils/pybind.h>
 
+#include <memory>
+#include <string>
 #include <utility>
 #include <vector>
 
@@ -443,10 +452,106 @@ PyObject* ClipGrads(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// embedding(tokens, weight, out_dtype, scale) -> rows; out_dtype < 0: the table's type
+// An error of the library on its way to Python, or to autograd.
+struct LibraryError {
+  int code;
+  std::string message;
+};
+void Want(bool ok, int code, const char* message) {
+  if (!ok) throw LibraryError{code, message};
+}
+void CheckCode(int code) {
+  if (code == 0) return;
+  std::string m = ibcomm_last_error();
+  while (!m.empty() && (m.back() == '\n' || m.back() == ' ')) m.pop_back();
+  throw LibraryError{code, m};
+}
+
+int FloatCode(const at::Tensor& t) {
+  const int d = DTypeCode(t.scalar_type());
+  if (d != 0 && d != 4 && d != 5) throw LibraryError{kNotSupported, std::string("no embedding of ") + c10::toString(t.scalar_type())};
+  return d;
+}
+
+// Without the GIL; `tokens` and `weight` contiguous.
+at::Tensor Lookup(const at::Tensor& tokens, const at::Tensor& weight, int out_dtype, double scale) {
+  const c10::Device device = weight.device();
+  const c10::cuda::CUDAGuard guard(device);
+  c10::SmallVector<int64_t, 8> sizes(tokens.sizes().begin(), tokens.sizes().end());
+  sizes.push_back(weight.size(1));
+  at::Tensor out = Empty(sizes, out_dtype == 0 ? c10::kFloat : out_dtype == 4 ? c10::kHalf : c10::kBFloat16, device);
+  CheckCode(ibcomm_embedding(tokens.const_data_ptr(), DTypeCode(tokens.scalar_type()), static_cast<size_t>(tokens.numel()), weight.const_data_ptr(),
+                             FloatCode(weight), static_cast<size_t>(weight.size(0)), static_cast<size_t>(weight.size(1)), out.data_ptr(), out_dtype, scale,
+                             c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+  return out;
+}
+
+// Without the GIL; all contiguous, on one GPU.
+void AddGradient(const at::Tensor& tokens, const at::Tensor& grad, const at::Tensor& out, int64_t padding, double scale, bool accumulate) {
+  Want(out.dim() == 2, kInvalidArgument, "a table has rows and columns");
+  const size_t count = static_cast<size_t>(tokens.numel()), rows = static_cast<size_t>(out.size(0)), width = static_cast<size_t>(out.size(1));
+  Want(grad.dim() >= 1 && grad.size(-1) == out.size(1) && static_cast<size_t>(grad.numel()) == count * width, kInvalidArgument,
+       "grad must hold a row of the table's width for every token");
+  Want(tokens.is_cuda() && tokens.device() == out.device() && grad.device() == out.device(), kInvalidArgument,
+       "tokens, grad and table must live on the same GPU");
+  const c10::Device device = out.device();
+  const c10::cuda::CUDAGuard guard(device);
+  size_t bytes = 0;
+  CheckCode(ibcomm_embedding_grad_work(count, rows, width, &bytes));
+  at::Tensor work;
+  if (bytes > 0) work = Empty({static_cast<int64_t>(bytes)}, c10::kByte, device);
+  CheckCode(ibcomm_embedding_grad(tokens.const_data_ptr(), DTypeCode(tokens.scalar_type()), count, grad.const_data_ptr(), FloatCode(grad), out.data_ptr(),
+                                  FloatCode(out), rows, width, padding, scale, accumulate ? 1 : 0, bytes > 0 ? work.data_ptr() : nullptr, bytes,
+                                  c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+}
+
+// The embedding's place in autograd's graph: the table's gradient, or with `into` its addition to that tensor.
+struct EmbeddingBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable tokens;
+  at::Tensor weight, into;
+  double scale = 1.0;
+  int64_t padding = -1;
+
+  std::string name() const override { return "EmbeddingBackward"; }
+  void release_variables() override {
+    tokens.reset_data();
+    released = true;
+  }
+  bool released = false;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    TORCH_CHECK(!released, "the embedding's gradient was taken already; specify retain_graph=True to take it again");
+    const at::Tensor& grad = grads[0];
+    if (!grad.defined()) return {at::Tensor()};
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()), "the embedding's gradient can be taken once, not differentiated again");
+    const at::NoGradGuard no_grad;
+    const at::Tensor ids = tokens.unpack(), rows = grad.contiguous();
+    try {
+      if (!into.defined()) {
+        at::Tensor out = at::empty(weight.sizes(), weight.options());
+        AddGradient(ids, rows, out, padding, scale, false);
+        return {out};
+      }
+      AddGradient(ids, rows, into, padding, scale, true);
+    } catch (const LibraryError& e) {
+      TORCH_CHECK(false, "[ibcomm error ", e.code, "] ", e.message);
+    }
+    // A gradient without entries costs nothing to add, and takes the way of every other one: autograd makes the stream
+    // of weight.grad wait for this one, adds other uses of the table and runs the bucket's hook, in that order.
+    if (weight.is_leaf() && weight.grad().defined()) return {at::empty(weight.sizes(), weight.options().layout(c10::kSparse))};
+    // Where nothing is handed on, the stream of the backward call waits at its end.
+    const c10::Device device = into.device();
+    auto done = std::make_shared<c10::Event>(c10::DeviceType::CUDA);
+    done->record(c10::cuda::getCurrentCUDAStream(device.index()).unwrap());
+    torch::autograd::Engine::get_default_engine().queue_callback([done, device] { done->block(c10::cuda::getCurrentCUDAStream(device.index()).unwrap()); });
+    return {at::Tensor()};
+  }
+};
+
+// embedding(tokens, weight, out_dtype, scale, padding_row, grad_into) -> rows; out_dtype < 0: the table's type
 PyObject* Embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!WantArgs(n, 4)) return nullptr;
+  if (!WantArgs(n, 6)) return nullptr;
   int dt, dw;
   const at::Tensor* tokens = Tensor(a[0], &dt);
   if (tokens == nullptr) return nullptr;
@@ -454,28 +559,38 @@ PyObject* Embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (weight == nullptr) return nullptr;
   const int wanted = static_cast<int>(PyLong_AsLong(a[2]));
   const double scale = PyFloat_AsDouble(a[3]);
+  const int64_t padding = PyLong_AsLongLong(a[4]);
   if (PyErr_Occurred()) return nullptr;
+  const at::Tensor* into = nullptr;
+  if (a[5] != Py_None) {
+    int d;
+    if ((into = Tensor(a[5], &d)) == nullptr) return nullptr;
+  }
   if (weight->dim() != 2) return Raise(kInvalidArgument, "a table has rows and columns");
   if (!tokens->is_cuda() || !weight->is_cuda() || tokens->device() != weight->device())
     return Raise(kInvalidArgument, "tokens and table must live on the same GPU");
   const int out_dtype = wanted < 0 ? dw : wanted;
   if (out_dtype != 0 && out_dtype != 4 && out_dtype != 5) return Raise(kNotSupported, "rows are float32, float16 or bfloat16");
-  const c10::Device device = weight->device();
-  const c10::cuda::CUDAGuard guard(device);
-  c10::SmallVector<int64_t, 8> sizes(tokens->sizes().begin(), tokens->sizes().end());
-  sizes.push_back(weight->size(1));
-  at::Tensor out = Empty(sizes, out_dtype == 0 ? c10::kFloat : out_dtype == 4 ? c10::kHalf : c10::kBFloat16, device);
-  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  const void* t = tokens->const_data_ptr();
-  const void* w = weight->const_data_ptr();
-  void* o = out.data_ptr();
-  const size_t count = static_cast<size_t>(tokens->numel()), rows = static_cast<size_t>(weight->size(0)), width = static_cast<size_t>(weight->size(1));
-  int code;
-  Py_BEGIN_ALLOW_THREADS;
-  code = ibcomm_embedding(t, dt, count, w, dw, rows, width, o, out_dtype, scale, stream);
-  Py_END_ALLOW_THREADS;
-  if (code != 0) return RaiseLast(code);
-  return THPVariable_Wrap(std::move(out));
+  try {
+    at::Tensor out;
+    {
+      const pybind11::gil_scoped_release unlocked;
+      out = Lookup(*tokens, *weight, out_dtype, scale);
+      if (at::GradMode::is_enabled() && weight->requires_grad()) {
+        const std::shared_ptr<EmbeddingBackward> node(new EmbeddingBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(*weight));
+        node->tokens = torch::autograd::SavedVariable(*tokens, false);
+        node->weight = *weight;
+        if (into != nullptr) node->into = *into;
+        node->scale = scale;
+        node->padding = padding;
+        torch::autograd::set_history(out, node);
+      }
+    }
+    return THPVariable_Wrap(std::move(out));
+  } catch (const LibraryError& e) {
+    return Raise(e.code, e.message.c_str());
+  }
   END_HANDLE_TH_ERRORS
 }
 
@@ -494,27 +609,13 @@ PyObject* EmbeddingGrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double scale = PyFloat_AsDouble(a[4]);
   const int accumulate = PyObject_IsTrue(a[5]);
   if (PyErr_Occurred()) return nullptr;
-  if (out->dim() != 2) return Raise(kInvalidArgument, "a table has rows and columns");
-  const size_t count = static_cast<size_t>(tokens->numel()), rows = static_cast<size_t>(out->size(0)), width = static_cast<size_t>(out->size(1));
-  if (grad->dim() < 1 || grad->size(-1) != out->size(1) || static_cast<size_t>(grad->numel()) != count * width)
-    return Raise(kInvalidArgument, "grad must hold a row of the table's width for every token");
-  if (!tokens->is_cuda() || !grad->is_cuda() || !out->is_cuda() || tokens->device() != out->device() || grad->device() != out->device())
-    return Raise(kInvalidArgument, "tokens, grad and table must live on the same GPU");
-  const c10::Device device = out->device();
-  const c10::cuda::CUDAGuard guard(device);
-  size_t bytes = 0;
-  int code = ibcomm_embedding_grad_work(count, rows, width, &bytes);
-  if (code != 0) return RaiseLast(code);
-  at::Tensor work = Empty({static_cast<int64_t>(bytes)}, c10::kByte, device);
-  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-  const void* t = tokens->const_data_ptr();
-  const void* g = grad->const_data_ptr();
-  void* o = out->data_ptr();
-  void* w = work.data_ptr();
-  Py_BEGIN_ALLOW_THREADS;
-  code = ibcomm_embedding_grad(t, dt, count, g, dg, o, dout, rows, width, padding, scale, accumulate, w, bytes, stream);
-  Py_END_ALLOW_THREADS;
-  return Done(code);
+  try {
+    const pybind11::gil_scoped_release unlocked;
+    AddGradient(*tokens, *grad, *out, padding, scale, accumulate != 0);
+  } catch (const LibraryError& e) {
+    return Raise(e.code, e.message.c_str());
+  }
+  Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 

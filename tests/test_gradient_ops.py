@@ -183,9 +183,9 @@ def test_what_the_call_path_refuses_of_cuda_tensors():
         "fast.clip_grads([t.reshape(2, 4)], [t.reshape(4, 2).t()], 2, 1.0, None)": "an output must match its tensor in shape and strides",
         "fast.clip_grads([t], [other], 2, 1.0, None)": "the tensors must live on one GPU",
         "fast.clip_grads([t], None, 2, 1.0, t)": "the ranks' sums must be float64 on the tensors' GPU",
-        "fast.embedding(host, t.reshape(2, 4), -1, 1.0)": "tensors must live on the GPU",
-        "fast.embedding(other, t.reshape(2, 4), -1, 1.0)": "tokens and table must live on the same GPU",
-        "fast.embedding(t, t, -1, 1.0)": "a table has rows and columns",
+        "fast.embedding(host, t.reshape(2, 4), -1, 1.0, -1, None)": "tensors must live on the GPU",
+        "fast.embedding(other, t.reshape(2, 4), -1, 1.0, -1, None)": "tokens and table must live on the same GPU",
+        "fast.embedding(t, t, -1, 1.0, -1, None)": "a table has rows and columns",
         "fast.embedding_grad(t, t, t, -1, 1.0, False)": "a table has rows and columns",
         "fast.embedding_grad(t[:3], t, t.reshape(2, 4), -1, 1.0, False)": "grad must hold a row of the table's width for every token",
         "fast.embedding_grad(other[:2], t.reshape(2, 4), t.reshape(2, 4), -1, 1.0, False)": "tokens, grad and table must live on the same GPU",
@@ -225,9 +225,9 @@ def test_what_the_c_interface_refuses():
     assert clip(grad_tensors((4096, 4096, 8, 0, 0), (4096 + 28, 4096 + 28, 8, 0, 0))) == ar.INVALID_ARGUMENT
 
     size = C.c_size_t(0)
-    assert lib.ibcomm_embedding_grad_work(100, 50, 64, C.byref(size)) == 0 and size.value > 0
-    assert lib.ibcomm_embedding_grad_work(100, 50, 64, None) == ar.INVALID_ARGUMENT
-    grad = lambda tok=1 << 20, td=3, n=100, g=1 << 21, gd=0, out=1 << 22, od=0, rows=50, width=64, pad=-1, s=1.0, work=1 << 23, b=size.value: (  # noqa: E731
+    assert lib.ibcomm_embedding_grad_work(1000, 50, 64, C.byref(size)) == 0 and size.value > 0
+    assert lib.ibcomm_embedding_grad_work(1000, 50, 64, None) == ar.INVALID_ARGUMENT
+    grad = lambda tok=1 << 20, td=3, n=1000, g=1 << 21, gd=0, out=1 << 22, od=0, rows=50, width=64, pad=-1, s=1.0, work=1 << 23, b=size.value: (  # noqa: E731
         lib.ibcomm_embedding_grad(tok, td, n, g, gd, out, od, rows, width, pad, s, 0, work, b, None))
     assert grad(td=0) == ar.NOT_SUPPORTED and grad(gd=1) == ar.NOT_SUPPORTED and grad(od=2) == ar.NOT_SUPPORTED
     assert grad(tok=None) == ar.INVALID_ARGUMENT and grad(g=None) == ar.INVALID_ARGUMENT and grad(out=None) == ar.INVALID_ARGUMENT
