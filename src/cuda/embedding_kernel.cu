@@ -557,7 +557,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   constexpr int kCols = S::kCols;
   __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
   __shared__ uint32_t before_key[kSumWarps], first_key[kSumWarps], last_key[kSumWarps], behind_key[kSumWarps];
-  __shared__ uint32_t run_first, run_last, is_last;
+  __shared__ uint32_t run_first[2], run_last[2], is_last[2];  // of the runs over the range's two edges
   const S slice(tile, p.width);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t i0 = (range * kSumWarps + warp) * p.per_warp;
@@ -592,6 +592,16 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
     for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
   };
   auto row = [&](int j) { return grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j & 31)) * p.width; };
+  // How far the runs over the range's edges reach, looked up while the first rows are on their way.
+  auto reach = [&](int side, uint32_t k) {
+    uint32_t a, b;
+    RangesOfRun(p, k, range, &a, &b);
+    if (lane == 0) run_first[side] = a, run_last[side] = b;
+  };
+  auto reaches = [&] {
+    if (warp == 0 && began_before && known > 0) reach(0, __shfl_sync(0xffffffffu, key, 0));
+    if (warp == kSumWarps - 1 && goes_on && known == count && count > 0) reach(1, __shfl_sync(0xffffffffu, key, count - 1));
+  };
   if constexpr (kVector) {
     constexpr int kSlot = S::kSlotBytes;
     unsigned char* mine = ring + warp * (S::kSlots * kSlot) + lane * S::kVecBytes;
@@ -602,6 +612,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
       if (u < known) slice.Fetch(r, mine_shared + u * kSlot);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    reaches();
     for (int j0 = 0; j0 < known; j0 += S::kSlots) {
 #pragma unroll
       for (int u = 0; u < S::kSlots; ++u) {
@@ -619,6 +630,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     constexpr int kTogether = 4;
+    reaches();
     for (int j0 = 0; j0 < known; j0 += kTogether) {
       TG v[kTogether][kCols];
 #pragma unroll
@@ -666,23 +678,18 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   const uint32_t end = last_key[kSumWarps - 1];
   const bool to_behind = end < p.rows && behind_key[kSumWarps - 1] == end && !(from_before && first_key[0] == end);
   if (!from_before && !to_behind) return;
-  __threadfence();
-  for (int side = from_before ? 0 : 1; side < (to_behind ? 2 : 1); ++side) {
-    const uint32_t row = side == 0 ? first_key[0] : end;
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t a, b;
-      RangesOfRun(p, row, range, &a, &b);
-      if (lane == 0) {
-        run_first = a;
-        run_last = b;
-        is_last = atomicAdd(p.arrived + static_cast<uint64_t>(a) * p.tiles + tile, 1u) == b - a;
-      }
-    }
-    __syncthreads();
-    if (!is_last) continue;
+  __syncthreads();
+  if (threadIdx.x < 2 && (threadIdx.x == 0 ? from_before : to_behind)) {
+    __threadfence();  // the block's parts are there before it counts as arrived
+    const uint32_t a = run_first[threadIdx.x];
+    is_last[threadIdx.x] = atomicAdd(p.arrived + static_cast<uint64_t>(a) * p.tiles + tile, 1u) == run_last[threadIdx.x] - a;
     __threadfence();
-    const uint32_t parts = run_last - run_first + 1;
+  }
+  __syncthreads();
+  for (int side = from_before ? 0 : 1; side < (to_behind ? 2 : 1); ++side) {
+    if (!is_last[side]) continue;
+    const uint32_t row = side == 0 ? first_key[0] : end;
+    const uint32_t parts = run_last[side] - run_first[side] + 1;
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(parts) * warp / kSumWarps);
     const uint32_t stop = static_cast<uint32_t>(static_cast<uint64_t>(parts) * (warp + 1) / kSumWarps);
 #pragma unroll
@@ -691,7 +698,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
     for (uint32_t i = begin; i < stop; ++i) {
       float a[kCols];
       // The run goes on behind its first range and began before the others.
-      slice.Load(p.partial + (2 * static_cast<uint64_t>(run_first + i) + (i == 0 ? 1 : 0)) * p.width, a);
+      slice.Load(p.partial + (2 * static_cast<uint64_t>(run_first[side] + i) + (i == 0 ? 1 : 0)) * p.width, a);
 #pragma unroll
       for (int e = 0; e < kCols; ++e) sum[e] += a[e];
     }
@@ -705,6 +712,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
       }
       WriteRow<TO>(p, slice, row, sum);
     }
+    __syncthreads();
   }
 }
 
