@@ -50,7 +50,9 @@ __device__ __forceinline__ void StoreValues(T* p, const float* a) {
 
 // ------------------------------------------------------------------ lookup
 constexpr int kLookupThreads = 256;
-constexpr int kLookupUnroll = 4;
+// Quanta of a lane: one value each, four would leave a warp with 8 bytes on their way per lane (16384 rows of 1001 fp32
+// into bf16: 28.8 us, with sixteen LOOKUP16 us).
+constexpr int LookupUnroll(bool vector) { return vector ? 4 : 16; }
 
 template <typename TI, typename TO>
 struct LookupQuantum {
@@ -70,20 +72,20 @@ __device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
 template <typename TI, typename TO, bool kTokens64, bool kVector>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
                                                                   uint64_t num_tokens, uint32_t per_row, uint32_t parts, int lanes, uint64_t rows, uint64_t width, float scale) {
-  constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1;
+  constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1, kUnroll = LookupUnroll(kVector);
   const uint32_t lane = threadIdx.x & 31, group = 1u << lanes;
   const uint32_t block = blockIdx.x / parts, part = blockIdx.x - block * parts;
   const uint64_t warp = static_cast<uint64_t>(block) * (kLookupThreads / 32) + threadIdx.x / 32;
   const uint64_t t = (warp << (5 - lanes)) + (lane >> lanes);
   if (t >= num_tokens) return;
-  const uint32_t first = (part * kLookupUnroll << lanes) + (lane & (group - 1));
+  const uint32_t first = (part * kUnroll << lanes) + (lane & (group - 1));
   const int64_t id = Token<kTokens64>(tokens, t);
   const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
   const TI* from = weight + (inside ? static_cast<uint64_t>(id) : 0) * width;
   TO* to = out + t * width;
-  float a[kLookupUnroll][kN];
+  float a[kUnroll][kN];
 #pragma unroll
-  for (int u = 0; u < kLookupUnroll; ++u) {
+  for (int u = 0; u < kUnroll; ++u) {
     const uint32_t q = first + (u << lanes);
 #pragma unroll
     for (int e = 0; e < kN; ++e) a[u][e] = 0.f;
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __
     }
   }
 #pragma unroll
-  for (int u = 0; u < kLookupUnroll; ++u) {
+  for (int u = 0; u < kUnroll; ++u) {
     const uint32_t q = first + (u << lanes);
     if (q < per_row) {
       if (inside) {  // a row that is not there is zero whatever the scale is
@@ -427,36 +429,57 @@ struct Slice {
   static constexpr int kPer = !kVector ? 1 : sizeof(TG) == 2 && sizeof(TO) == 2 ? 8 : 4;  // adjacent columns
   static constexpr int kVecs = kCols / kPer;
   static constexpr int kVecBytes = kPer * static_cast<int>(sizeof(TG));
-  static constexpr int kSlotBytes = 32 * kCols * static_cast<int>(sizeof(TG));
-  static constexpr int kSlots = 4096 / kSlotBytes;  // rows on their way to a warp
-  static constexpr int kRing = kVector ? kSumWarps * kSlots * kSlotBytes : 0;
+  static constexpr int kRowBytes = 32 * kCols * static_cast<int>(sizeof(TG));
+  static constexpr int kSlotBytes = kRowBytes + (kVector ? 0 : 16);
+  static constexpr int kSlots = 4096 / kRowBytes;  // rows on their way to a warp
+  static constexpr int kRing = kSumWarps * kSlots * kSlotBytes;
   uint64_t width;
   uint64_t column;  // the lane's first; the others are 32 * kPer apart
   __device__ __forceinline__ Slice(uint32_t tile, uint64_t w) : width(w), column(static_cast<uint64_t>(tile) * (32 * kCols) + (threadIdx.x & 31) * kPer) {}
   // With kVector the width is a multiple of kPer: a lane has all columns of a vector or none.
   __device__ __forceinline__ bool Has(int v) const { return column + v * (32 * kPer) < width; }
 
-  // A row into one of the warp's slots, without waiting for it; a lane reads what it has written itself.
+  // A row into one of the warp's slots (`slot`: its start), without waiting for it.  With kVector a lane copies what it
+  // reads itself.  Else the warp copies the 16-byte words of memory that hold the slice: no allocation ends inside one,
+  // and a row may start at any element of one.
   __device__ __forceinline__ void Fetch(const TG* row, unsigned slot) const {
+    const int lane = threadIdx.x & 31;
+    if constexpr (kVector) {
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-      if (Has(v)) {
-        const TG* from = row + column + v * (32 * kPer);
-        if constexpr (kVecBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + v * 512), "l"(from) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(slot + v * 256), "l"(from) : "memory");
+      for (int v = 0; v < kVecs; ++v) {
+        if (Has(v)) {
+          const TG* from = row + column + v * (32 * kPer);
+          const unsigned to = slot + (v * 32 + lane) * kVecBytes;
+          if constexpr (kVecBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+        }
       }
+    } else {
+      const uint64_t first = column - lane, columns = min(width - first, static_cast<uint64_t>(32 * kCols));
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(row + first), end = begin + columns * sizeof(TG);
+#pragma unroll
+      for (int v = 0; v < kRowBytes / 512 + 1; ++v) {
+        const uintptr_t from = begin / 16 * 16 + (v * 32 + lane) * 16;
+        if (from < end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (v * 32 + lane) * 16), "l"(from) : "memory");
+      }
+    }
   }
-  __device__ __forceinline__ void AddSlot(const unsigned char* slot, float* sum) const {
+  __device__ __forceinline__ void AddSlot(const TG* row, const unsigned char* slot, float* sum) const {
+    const int lane = threadIdx.x & 31;
+    const unsigned char* at = slot + lane * kVecBytes;
+    if constexpr (!kVector) at += reinterpret_cast<uintptr_t>(row + (column - lane)) % 16;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
       if constexpr (kVecBytes == 16) {
-        VecIO<TG>::Add(*reinterpret_cast<const uint4*>(slot + v * 512), sum + v * kPer);
-      } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(slot + v * 256);
+        VecIO<TG>::Add(*reinterpret_cast<const uint4*>(at + v * 512), sum + v * kPer);
+      } else if constexpr (kPer == 4) {
+        const uint2 q = *reinterpret_cast<const uint2*>(at + v * 256);
         float a[8];
         VecIO<TG>::Load(make_uint4(q.x, q.y, 0, 0), a);
 #pragma unroll
         for (int e = 0; e < kPer; ++e) sum[v * kPer + e] += a[e];
+      } else {
+        if (Has(v)) sum[v] += ToAcc<float, TG>(*reinterpret_cast<const TG*>(at + v * 32 * sizeof(TG)));
       }
     }
   }
@@ -602,53 +625,33 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
     if (warp == 0 && began_before && known > 0) reach(0, __shfl_sync(0xffffffffu, key, 0));
     if (warp == kSumWarps - 1 && goes_on && known == count && count > 0) reach(1, __shfl_sync(0xffffffffu, key, count - 1));
   };
-  if constexpr (kVector) {
-    constexpr int kSlot = S::kSlotBytes;
-    unsigned char* mine = ring + warp * (S::kSlots * kSlot) + lane * S::kVecBytes;
-    const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
+  constexpr int kSlot = S::kSlotBytes;
+  unsigned char* mine = ring + warp * (S::kSlots * kSlot);
+  const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
+#pragma unroll
+  for (int u = 0; u < S::kSlots; ++u) {
+    const TG* r = row(u);
+    if (u < known) slice.Fetch(r, mine_shared + u * kSlot);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  reaches();
+  for (int j0 = 0; j0 < known; j0 += S::kSlots) {
 #pragma unroll
     for (int u = 0; u < S::kSlots; ++u) {
-      const TG* r = row(u);
-      if (u < known) slice.Fetch(r, mine_shared + u * kSlot);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    reaches();
-    for (int j0 = 0; j0 < known; j0 += S::kSlots) {
-#pragma unroll
-      for (int u = 0; u < S::kSlots; ++u) {
-        const int j = j0 + u;
-        if (j < known) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
-          slice.AddSlot(mine + u * kSlot, sum);
-          const TG* r = row(j + S::kSlots);
-          if (j + S::kSlots < known) slice.Fetch(r, mine_shared + u * kSlot);
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (ends >> j & 1) flush(j);
-        }
-      }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-  } else {
-    constexpr int kTogether = 4;
-    reaches();
-    for (int j0 = 0; j0 < known; j0 += kTogether) {
-      TG v[kTogether][kCols];
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        const TG* r = row(j0 + u);
-#pragma unroll
-        for (int e = 0; e < kCols; ++e) v[u][e] = j0 + u < known && slice.Has(e) ? r[slice.column + e * 32] : FromAcc<TG, float>(0.f);
-      }
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u) {
-        if (j0 + u < known) {
-#pragma unroll
-          for (int e = 0; e < kCols; ++e) sum[e] += ToAcc<float, TG>(v[u][e]);
-          if (ends >> (j0 + u) & 1) flush(j0 + u);
-        }
+      const int j = j0 + u;
+      if (j < known) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
+        if constexpr (!kVector) __syncwarp();  // what the other lanes have copied
+        slice.AddSlot(row(j), mine + u * kSlot, sum);
+        if constexpr (!kVector) __syncwarp();  // they have read it
+        const TG* r = row(j + S::kSlots);
+        if (j + S::kSlots < known) slice.Fetch(r, mine_shared + u * kSlot);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (ends >> j & 1) flush(j);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (lane == 0) {
     before_key[warp] = before;
     first_key[warp] = key;
@@ -717,7 +720,7 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
 }
 
 template <typename TG, typename TO, bool kVector>
-__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) SumRunsKernel(SumParams p) {
+__global__ void __launch_bounds__(kSumThreads, 4) SumRunsKernel(SumParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   WaitForPrevious();
   const uint32_t range = blockIdx.x / p.tiles;
@@ -739,7 +742,7 @@ struct SmallParams {
 };
 
 template <typename TG, typename TO, bool kVector>
-__global__ void __launch_bounds__(kSumThreads, kVector ? 4 : 2) FewTokensKernel(SmallParams p) {
+__global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ __align__(16) uint32_t keys[kSmallTokens], sorted[kSmallTokens], positions[kSmallTokens], named[kClearRows / 32];
   const uint32_t t = threadIdx.x, n = p.sum.n;
@@ -803,7 +806,8 @@ cudaError_t LaunchLookup(const EmbeddingParams& p, cudaStream_t stream) {
   while (lanes < 5 && (1ull << lanes) < per_row) ++lanes;
   const uint64_t per_block = static_cast<uint64_t>(dev::kLookupThreads) >> lanes;
   const uint64_t blocks = (p.num_tokens + per_block - 1) / per_block;
-  const uint64_t parts = (per_row + (dev::kLookupUnroll << lanes) - 1) / (dev::kLookupUnroll << lanes);
+  const uint64_t quanta = static_cast<uint64_t>(dev::LookupUnroll(vector)) << lanes;
+  const uint64_t parts = (per_row + quanta - 1) / quanta;
   if (blocks * parts > 0x7fffffffull) return cudaErrorInvalidValue;
   const TI* w = static_cast<const TI*>(p.weight);
   TO* o = static_cast<TO*>(p.out);
@@ -1035,14 +1039,14 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
         kernel<<<static_cast<unsigned>(blocks), dev::kSumThreads, ring, stream>>>(small);
         return cudaGetLastError();
       };
-      return vector ? launch(dev::FewTokensKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::FewTokensKernel<TG, TO, false>, 0);
+      return vector ? launch(dev::FewTokensKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::FewTokensKernel<TG, TO, false>, dev::Slice<TG, TO, false>::kRing);
     }
     auto launch = [&](auto kernel, int ring) {
       const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
       if (e != cudaSuccess) return e;
       return LaunchEarly(kernel, grid, dev::kSumThreads, static_cast<size_t>(ring), stream, sum);
     };
-    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, 0);
+    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, dev::Slice<TG, TO, false>::kRing);
   });
 }
 
