@@ -50,9 +50,8 @@ __device__ __forceinline__ void StoreValues(T* p, const float* a) {
 
 // ------------------------------------------------------------------ lookup
 constexpr int kLookupThreads = 256;
-// Quanta of a lane: one value each, four would leave a warp with 8 bytes on their way per lane (16384 rows of 1001 fp32
-// into bf16: 28.8 us, with sixteen LOOKUP16 us).
-constexpr int LookupUnroll(bool vector) { return vector ? 4 : 16; }
+constexpr int kLookupUnroll = 4;
+constexpr int kLookupColumns = 512;  // of a warp, where rows do not come in vectors
 
 template <typename TI, typename TO>
 struct LookupQuantum {
@@ -66,45 +65,86 @@ __device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
   else return static_cast<const int*>(tokens)[t];
 }
 
-// A warp takes kUnroll * 32 quanta of a row (kN values with kVector, else one),
-// all loads before the first store; where a row has fewer than 32, 1 << lanes of
-// the warp's lanes take a row each.  The parts of a row are neighbours in the grid.
-template <typename TI, typename TO, bool kTokens64, bool kVector>
+// A warp takes kLookupUnroll * 32 quanta (kN values each) of a row, all loads
+// before the first store; where a row has fewer than 32, 1 << lanes of the warp's
+// lanes take a row each.  The parts of a row are neighbours in the grid.
+template <typename TI, typename TO, bool kTokens64>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
-                                                                  uint64_t num_tokens, uint32_t per_row, uint32_t parts, int lanes, uint64_t rows, uint64_t width, float scale) {
-  constexpr int kN = kVector ? LookupQuantum<TI, TO>::kN : 1, kUnroll = LookupUnroll(kVector);
+                                                                  uint64_t num_tokens, uint32_t per_row, uint32_t parts, int lanes, uint64_t rows, uint64_t width,
+                                                                  float scale) {
+  constexpr int kN = LookupQuantum<TI, TO>::kN;
   const uint32_t lane = threadIdx.x & 31, group = 1u << lanes;
   const uint32_t block = blockIdx.x / parts, part = blockIdx.x - block * parts;
   const uint64_t warp = static_cast<uint64_t>(block) * (kLookupThreads / 32) + threadIdx.x / 32;
   const uint64_t t = (warp << (5 - lanes)) + (lane >> lanes);
   if (t >= num_tokens) return;
-  const uint32_t first = (part * kUnroll << lanes) + (lane & (group - 1));
+  const uint32_t first = (part * kLookupUnroll << lanes) + (lane & (group - 1));
   const int64_t id = Token<kTokens64>(tokens, t);
   const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
   const TI* from = weight + (inside ? static_cast<uint64_t>(id) : 0) * width;
   TO* to = out + t * width;
-  float a[kUnroll][kN];
+  float a[kLookupUnroll][kN];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kLookupUnroll; ++u) {
     const uint32_t q = first + (u << lanes);
 #pragma unroll
     for (int e = 0; e < kN; ++e) a[u][e] = 0.f;
-    if (inside && q < per_row) {
-      if constexpr (kVector) LoadValues<TI, kN>(from + static_cast<uint64_t>(q) * kN, a[u]);
-      else a[u][0] = ToAcc<float, TI>(from[q]);
-    }
+    if (inside && q < per_row) LoadValues<TI, kN>(from + static_cast<uint64_t>(q) * kN, a[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < kLookupUnroll; ++u) {
     const uint32_t q = first + (u << lanes);
     if (q < per_row) {
       if (inside) {  // a row that is not there is zero whatever the scale is
 #pragma unroll
         for (int e = 0; e < kN; ++e) a[u][e] *= scale;
       }
-      if constexpr (kVector) StoreValues<TO, kN>(to + static_cast<uint64_t>(q) * kN, a[u]);
-      else to[q] = FromAcc<TO, float>(a[u][0]);
+      StoreValues<TO, kN>(to + static_cast<uint64_t>(q) * kN, a[u]);
     }
+  }
+}
+
+// Rows that do not come in vectors, because of their width or of where they
+// start: a warp copies the 16-byte words of memory that hold its columns into
+// shared memory (no allocation ends inside one) and stores 16-bit values in pairs.
+template <typename TI, typename TO, bool kTokens64>
+__global__ void __launch_bounds__(kLookupThreads) EmbeddingRaggedKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
+                                                                        uint64_t num_tokens, uint32_t parts, uint64_t rows, uint64_t width, float scale) {
+  constexpr int kBytes = kLookupColumns * static_cast<int>(sizeof(TI)) + 16;
+  __shared__ __align__(16) unsigned char memory[kLookupThreads / 32][kBytes];
+  const int lane = threadIdx.x & 31;
+  unsigned char* mine = memory[threadIdx.x / 32];
+  const uint32_t block = blockIdx.x / parts, part = blockIdx.x - block * parts;
+  const uint64_t t = static_cast<uint64_t>(block) * (kLookupThreads / 32) + threadIdx.x / 32;
+  if (t >= num_tokens) return;
+  const uint64_t first = static_cast<uint64_t>(part) * kLookupColumns;
+  const int columns = static_cast<int>(min(width - first, static_cast<uint64_t>(kLookupColumns)));
+  const int64_t id = Token<kTokens64>(tokens, t);
+  const bool inside = id >= 0 && static_cast<uint64_t>(id) < rows;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(weight + (inside ? static_cast<uint64_t>(id) : 0) * width + first);
+  const TI* row = reinterpret_cast<const TI*>(mine + begin % 16);
+  if (inside) {
+    const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(mine));
+    const uintptr_t end = begin + columns * sizeof(TI);
+#pragma unroll
+    for (int v = 0; v < kLookupColumns * static_cast<int>(sizeof(TI)) / 512 + 1; ++v) {
+      const uintptr_t from = begin / 16 * 16 + (v * 32 + lane) * 16;
+      if (from < end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (v * 32 + lane) * 16), "l"(from) : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  __syncwarp();
+  auto value = [&](int c) { return inside ? ToAcc<float, TI>(row[c]) * scale : 0.f; };
+  TO* to = out + t * width + first;
+  if constexpr (sizeof(TO) == 4) {
+    for (int c = lane; c < columns; c += 32) to[c] = value(c);
+  } else {
+    const int head = reinterpret_cast<uintptr_t>(to) / 2 % 2;  // values before the first pair
+    if (lane == 0 && head > 0) to[0] = FromAcc<TO, float>(value(0));
+    const int pairs = (columns - head) / 2;
+#pragma unroll 4
+    for (int q = lane; q < pairs; q += 32) *reinterpret_cast<unsigned*>(to + head + 2 * q) = VecIO<TO>::P2(value(head + 2 * q), value(head + 2 * q + 1));
+    if (lane == 0 && head + 2 * pairs < columns) to[columns - 1] = FromAcc<TO, float>(value(columns - 1));
   }
 }
 
@@ -801,21 +841,26 @@ cudaError_t LaunchLookup(const EmbeddingParams& p, cudaStream_t stream) {
   constexpr int kN = dev::LookupQuantum<TI, TO>::kN;
   auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
   const bool vector = p.width % kN == 0 && aligned(p.weight, kN * sizeof(TI)) && aligned(p.out, kN * sizeof(TO));
-  const uint64_t per_row = vector ? p.width / kN : p.width;
-  int lanes = 0;
-  while (lanes < 5 && (1ull << lanes) < per_row) ++lanes;
-  const uint64_t per_block = static_cast<uint64_t>(dev::kLookupThreads) >> lanes;
-  const uint64_t blocks = (p.num_tokens + per_block - 1) / per_block;
-  const uint64_t quanta = static_cast<uint64_t>(dev::LookupUnroll(vector)) << lanes;
-  const uint64_t parts = (per_row + quanta - 1) / quanta;
-  if (blocks * parts > 0x7fffffffull) return cudaErrorInvalidValue;
   const TI* w = static_cast<const TI*>(p.weight);
   TO* o = static_cast<TO*>(p.out);
-  const unsigned grid = static_cast<unsigned>(blocks * parts);
-  const uint32_t row = static_cast<uint32_t>(per_row);
   const float scale = static_cast<float>(p.scale);
-  if (vector) dev::EmbeddingKernel<TI, TO, kTokens64, true><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, static_cast<uint32_t>(parts), lanes, p.rows, p.width, scale);
-  else dev::EmbeddingKernel<TI, TO, kTokens64, false><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, row, static_cast<uint32_t>(parts), lanes, p.rows, p.width, scale);
+  int lanes = 0;
+  if (vector)
+    while (lanes < 5 && (1ull << lanes) < p.width / kN) ++lanes;
+  else lanes = 5;
+  const uint64_t per_block = static_cast<uint64_t>(dev::kLookupThreads) >> lanes;
+  const uint64_t blocks = (p.num_tokens + per_block - 1) / per_block;
+  const uint64_t columns = vector ? (static_cast<uint64_t>(dev::kLookupUnroll) << lanes) * kN : dev::kLookupColumns;
+  const uint64_t parts = (p.width + columns - 1) / columns;
+  if (blocks * parts > 0x7fffffffull) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(blocks * parts);
+  if (vector) {
+    dev::EmbeddingKernel<TI, TO, kTokens64><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, static_cast<uint32_t>(p.width / kN),
+                                                                                     static_cast<uint32_t>(parts), lanes, p.rows, p.width, scale);
+  } else {
+    dev::EmbeddingRaggedKernel<TI, TO, kTokens64><<<grid, dev::kLookupThreads, 0, stream>>>(p.tokens, w, o, p.num_tokens, static_cast<uint32_t>(parts), p.rows,
+                                                                                           p.width, scale);
+  }
   return cudaGetLastError();
 }
 
