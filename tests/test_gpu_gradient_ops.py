@@ -245,6 +245,33 @@ def test_two_streams_and_two_graphs_at_once():
             within(o, w, 7.5 * U * w.abs())
 
 
+@pytest.mark.parametrize("n", [700, 300000, 40000000])
+@pytest.mark.parametrize("power", [2.0, math.inf])
+def test_lists_of_every_size_in_a_graph(n, power):
+    # One cluster, the kernel that holds what it read, and the two kernels of long lists.
+    xs = [values((n,), F32, 1), values((n // 3,), BF16, 2)]
+    outs = [torch.empty_like(x) for x in xs]
+    ar.ops.clip_grad_norm(xs, 1.0, out=outs, norm_type=power)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ar.ops.grad_norm(xs, norm_type=power)
+        clipped = ar.ops.clip_grad_norm(xs, 1.0, out=outs, norm_type=power)
+        after = ar.ops.clip_grad_norm(outs, 0.5, norm_type=power)
+    for x in xs:
+        x.mul_(3)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    want = norm_of(xs, power).item()
+    within(norm, torch.tensor(want, device="cuda"), norm_rtol(F32) * want)
+    within(clipped, norm, 2 * norm_rtol(F32) * want)
+    # The second clipping sees the first one's values, rounded to bf16 here and there.
+    within(after, torch.ones((), device="cuda"), half(BF16) + 8 * U)
+    for x, o in zip(xs, outs):
+        w = x.double() * (0.5 / (want + 1e-6))
+        within(o, w, (3 * half(BF16) + 20 * U) * w.abs() + 2 * least(x.dtype))
+
+
 class TwoRanks:
     """What a communicator of two ranks does for the norm, seen from the first; `other` is the second's sum."""
     world_size, rank = 2, 0
@@ -443,6 +470,20 @@ def test_gradient_has_the_same_bits_every_time():
         assert torch.equal(ar.ops.embedding_grad(t, g, num_rows=500, dtype=F32), first)
 
 
+@pytest.mark.parametrize("n", [200, 5000, 30000, 40000])
+def test_tables_of_many_rows(n):
+    # Row numbers of 28 bits: three digits of the sort.
+    rows = (1 << 27) + 3
+    t = tokens_of(n, rows, n)
+    t[:3] = torch.tensor([rows - 1, 0, rows - 1])
+    g = torch.arange(1, n + 1, device="cuda", dtype=F32)[:, None] % 64
+    out = torch.zeros(rows, 1, device="cuda", dtype=F32)
+    ar.ops.embedding_grad(t, g, out=out, accumulate=True)
+    inside = (t >= 0) & (t < rows)
+    want = torch.zeros(rows, 1, device="cuda", dtype=F32).index_add_(0, t[inside], g[inside])  # whole numbers, exact
+    assert torch.equal(out, want)
+
+
 def test_largest_offsets():
     # More than 2^31 elements in the table and in the rows: a wide table whose last rows are named.
     rows, width = 270000, 8192
@@ -477,6 +518,32 @@ def test_gradient_through_autograd(table, rows_type):
     within(w.grad, want, (U * 300 + 3 * half(table)) * want.abs())
     with torch.no_grad():
         assert not ar.ops.embedding(t, w).requires_grad
+
+
+def test_what_autograd_refuses():
+    w = values((20, 8), F32, 1).requires_grad_(True)
+    t = tokens_of(30, 20, 2)
+    y = ar.ops.embedding(t, w)
+    dy = torch.ones_like(y).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(y, w, dy, create_graph=True, retain_graph=True)
+    (g,) = torch.autograd.grad(y, w, dy, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], g)
+    with pytest.raises(RuntimeError, match="retain_graph"):
+        torch.autograd.grad(y, w, dy)
+    y = ar.ops.embedding(t, w)
+    t.zero_()  # what the backward pass needs has changed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = ar.ops.embedding(t, w, grad_into=torch.zeros(20, 8, device="cuda", dtype=F16))
+    y.sum().backward()
+    assert w.grad is None
+    # No tokens at all, and a table that is no leaf.
+    ar.ops.embedding(t[:0], w).sum().backward()
+    assert w.grad.shape == w.shape and not w.grad.any()
+    half_table = w.detach().requires_grad_(True)
+    ar.ops.embedding(t, half_table * 2).sum().backward()
+    assert torch.equal(half_table.grad, 2 * grad_in_64_bits(t, torch.ones(30, 8, device="cuda"), 20, 1.0)[0].float())
 
 
 def test_gradient_against_differences():
