@@ -9,8 +9,9 @@ a synthetic batch, averages them over the ranks through
 SGD step.  With `--sharded` the averaging is a reduce-scatter, every rank
 updates only its block of the flat parameters, and an all-gather puts the
 parameters together again (the ZeRO-1 pattern).  With `--overlap` the allreduce
-of a bucket starts from an autograd hook while backward is still running.  At the end the ranks compare
-a checksum of their parameters: they must agree.
+of a bucket starts from an autograd hook while backward is still running.  With `--clip N` the averaged
+gradients are scaled so that the norm of all of them (over the ranks' blocks with `--sharded`) is at most N.
+At the end the ranks compare a checksum of their parameters: they must agree.
 
     python -m torch.distributed.run --nproc-per-node 8 examples/ddp_gradient_buckets.py
     python -m torch.distributed.run --nproc-per-node 2 examples/ddp_gradient_buckets.py --device cpu --sharded
@@ -40,6 +41,7 @@ def main() -> int:
     ap.add_argument("--sharded", action="store_true", help="reduce-scatter + sharded update + all-gather")
     ap.add_argument("--overlap", action="store_true",
                     help="start a bucket's allreduce from an autograd hook as soon as its gradients are complete")
+    ap.add_argument("--clip", type=float, default=0.0, help="largest norm of the averaged gradients (0: not clipped)")
     ap.add_argument("--hidden", type=int, default=256)
     args = ap.parse_args()
 
@@ -88,6 +90,8 @@ def main() -> int:
         loss.backward()
         if args.sharded:
             my_grads = grads.reduce_scatter(average=True, sync=True)
+            if args.clip > 0:
+                grads.clip_grad_norm(args.clip, sharded=True)
             for w, g in zip(weights.shards(), my_grads):
                 w.add_(g, alpha=-lr)          # this rank's block of the weights only
             weights.all_gather(sync=True)
@@ -96,6 +100,8 @@ def main() -> int:
                 grads.finish()                # the collectives were started during backward
             else:
                 grads.allreduce(average=True, sync=True)
+            if args.clip > 0:
+                grads.clip_grad_norm(args.clip)
             with torch.no_grad():
                 for p in params:
                     p.add_(p.grad, alpha=-lr)

@@ -122,6 +122,16 @@ def test_norm_of_shards_on_several_ranks(bins, np_, tmp_path):
     assert p.returncode == 0, p.stderr[-3000:]
 
 
+@pytest.mark.parametrize("mode", [[], ["--overlap"], ["--sharded"]])
+def test_example_with_clipping(mode):
+    port = 29660 + len(mode) + mode.count("--sharded")
+    cmd = ["timeout", "300s", sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2", "--master-addr", "127.0.0.1",
+           "--master-port", str(port), str(ROOT / "examples" / "ddp_gradient_buckets.py"), "--device", "cpu", "--steps", "2", "--clip", "0.1", *mode]
+    p = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert p.returncode == 0, p.stdout[-3000:]
+    assert p.stdout.count(": OK") == 2, p.stdout[-3000:]
+
+
 def code_of(call):
     with pytest.raises(ar.IbcommError) as e:
         call()
