@@ -8,6 +8,15 @@
 // written at once, one over its edges is joined in shared memory, one over the
 // range's edges in the workspace by the block that arrives last.  Every sum is
 // added in the tokens' order: the result does not depend on that of execution.
+//
+// All of it is bound by memory: a row is read once, a row of the table written
+// once (and read once where it is added to).  On a B200 (6.56 TB/s for a plain
+// copy), as calls among others, floors in brackets:
+//   lookup, 16384 rows of 2048 fp32 into bf16              22.5 us  (17.6)
+//   16384 rows of 4096 bf16 into an fp32 table of 50021    75 us    (50), 11 of them the sort, 57 the sums
+//   8192 rows of 2048 bf16 into a new table of 100003      73.5 us  (67.5), the sort hidden behind the clearing
+//   131072 rows of 1024 fp32 into an fp32 table of 32000   149 us   (121), 22 of them the sort, 127 the sums
+//   33 rows of 770 bf16 into an fp32 table                 6.2 us, the launch and a chain of four memory latencies
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -67,7 +76,9 @@ __device__ __forceinline__ int64_t Token(const void* tokens, uint64_t t) {
 
 // A warp takes kLookupUnroll * 32 quanta (kN values each) of a row, all loads
 // before the first store; where a row has fewer than 32, 1 << lanes of the warp's
-// lanes take a row each.  The parts of a row are neighbours in the grid.
+// lanes take a row each.  The parts of a row are neighbours in the grid.  Against
+// a thread per quantum, which divides to find its row: 26.7 -> 22.5 us for 16384
+// rows of 2048 fp32 into bf16; two or eight quanta per lane are the same.
 template <typename TI, typename TO, bool kTokens64>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
                                                                   uint64_t num_tokens, uint32_t per_row, uint32_t parts, int lanes, uint64_t rows, uint64_t width,
@@ -107,6 +118,7 @@ __global__ void __launch_bounds__(kLookupThreads) EmbeddingKernel(const void* __
 // Rows that do not come in vectors, because of their width or of where they
 // start: a warp copies the 16-byte words of memory that hold its columns into
 // shared memory (no allocation ends inside one) and stores 16-bit values in pairs.
+// 16384 rows of 4095 fp32 into bf16: 107 us value by value, 54 so (4096: 41).
 template <typename TI, typename TO, bool kTokens64>
 __global__ void __launch_bounds__(kLookupThreads) EmbeddingRaggedKernel(const void* __restrict__ tokens, const TI* __restrict__ weight, TO* __restrict__ out,
                                                                         uint64_t num_tokens, uint32_t parts, uint64_t rows, uint64_t width, float scale) {
@@ -193,6 +205,8 @@ __device__ __forceinline__ uint32_t KeyOf(const SortParams& p, uint32_t t) {
 // A least-significant-digit radix sort, cooperative: a block's part of the list
 // is cut into one part per warp, a digit's count of every warp gives the places.
 // A warp places 32 elements at a time in their order, so every pass is stable.
+// Equal digits in a warp are found by one ballot per bit (in the cluster's kernel,
+// 16384 tokens, 14.1 us against 16.2 with `match.any`).  131072 tokens of 32000 rows: 24 us, two digits of 8 bits.
 __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
   extern __shared__ uint32_t warp_counts[];  // kSortWarps x bins
   LetNextStart();
@@ -300,7 +314,10 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 // The same within one thread-block cluster, for lists that fit into its shared
 // memory: a thread holds kItems elements in registers, counts go from block to
 // block through distributed shared memory, elements are placed in the shared
-// memory of the block that has them in the next pass.
+// memory of the block that has them in the next pass.  Against the cooperative
+// kernel, tokens of 50000 rows: 2048 8.5 us against 18.5, 16384 13.5 against 22,
+// 32768 20.3 against 22.2, 65536 35 against 23 (there are only eight SMs to place
+// the elements), so lists of up to 32768 are taken.
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterBlocks = 8;  // at most
@@ -418,7 +435,7 @@ constexpr uint64_t kClearBytes = static_cast<uint64_t>(kClearThreads) * kClearUn
 
 // out = 0.  It reads nothing, so it runs beside the sort, on the SMs that the sort
 // leaves; its last block waits for the sort, so that whoever waits for this kernel
-// has waited for both.
+// has waited for both.  A table of 100003 x 2048 bf16: 56 us, 7.3 TB/s.
 __global__ void __launch_bounds__(kClearThreads) ClearKernel(unsigned char* out, uint64_t bytes) {
   LetNextStart();
   const uint64_t head = min(static_cast<uint64_t>((32 - reinterpret_cast<uintptr_t>(out) % 32) % 32), bytes);
@@ -440,7 +457,7 @@ __global__ void __launch_bounds__(kClearThreads) ClearKernel(unsigned char* out,
 // -------------------------------------------------------------------- sums
 constexpr int kSumWarps = 8;
 constexpr int kSumThreads = 32 * kSumWarps;
-constexpr int kMostWarpTokens = 16;
+constexpr int kMostWarpTokens = 16;  // with 8 or 32, 16384 rows of 4096 take 82 or 77 us instead of 75
 constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct SumParams {
@@ -462,7 +479,10 @@ struct SumParams {
 
 // A warp's slice of a row: 256 columns, eight per lane: with kVector in vectors
 // of at most 16 bytes of either type (a warp's access is one stretch of memory in
-// both), else one by one.
+// both: with 32 bytes of fp32 per lane 16384 bf16 rows of 4096 took 67 us instead
+// of 57), else one by one.  Rows come through a ring in shared memory, 4 KiB per
+// warp and 128 KiB per SM; in registers the same bytes left room for three blocks
+// per SM instead of four, and 131072 fp32 rows of 1024 took 180 us instead of 130.
 template <typename TG, typename TO, bool kVector>
 struct Slice {
   static constexpr int kCols = 8;
@@ -546,7 +566,8 @@ struct Slice {
       }
     }
   }
-  // Added by the memory: nothing to wait for.  Only one warp adds to a row, once.
+  // Added by the memory: nothing to wait for (16384 bf16 rows into fp32 75 us; loaded, added and stored 85).  Only one warp
+  // adds to a row, once.  These additions take subnormal numbers (below 1.2e-38) for zero.
   __device__ __forceinline__ void Add(float* row, const float* a) const {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -769,7 +790,8 @@ __global__ void __launch_bounds__(kSumThreads, 4) SumRunsKernel(SumParams p) {
 
 // Few tokens: every block sorts them all, by counting for each how many come
 // before it, and adds in its slice of the columns.  The blocks behind clear rows
-// that no token names.
+// that no token names.  One launch: 33 rows of 768 bf16 3.3 us on the device
+// against 11 with the kernels above, 256 rows 11.1 against 11.2, where it ends.
 constexpr uint32_t kSmallTokens = kSumThreads;
 constexpr uint32_t kClearRows = 8192;  // of a block, at most
 
