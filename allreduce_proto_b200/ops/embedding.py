@@ -52,7 +52,8 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, *, out: Optional[to
     where ``tokens`` is ``v``.
 
     ``out`` (contiguous, ``(rows, width)``) is overwritten, rows without tokens with zeros; with ``accumulate`` the sums
-    are added to it and only rows that tokens name are touched.  Without ``out`` a table of ``num_rows`` rows in ``dtype``
+    are added to it and only rows that tokens name are touched (in float32 tables subnormal numbers, below 1.2e-38, are
+    added as zero).  Without ``out`` a table of ``num_rows`` rows in ``dtype``
     (default: ``grad``'s) is made.  Types float32, float16, bfloat16 in any mixture; sums in float32, rounded once.
     ``tokens`` and ``grad`` may come from several ranks (``all_gather`` both): with many rows that few tokens name, that is
     less to send than the table's gradient."""

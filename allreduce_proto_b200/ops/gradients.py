@@ -2,8 +2,9 @@
 
 The norm is that of all tensors taken as one vector.  CUDA tensors: one pass over the gradients for the norm, one more
 where something is to be scaled; nothing is read back to the host, so the calls can be captured in a CUDA graph.  Sums are
-kept in float64 and joined in a fixed order: ranks with the same gradients get the same norm.  CPU tensors (float32,
-float64) are handled by the host library."""
+kept in float64 and joined in a fixed order: ranks with the same gradients in tensors of the same layout (sizes, order,
+addresses modulo 32 bytes, as in gradient buckets) get the same bits.  CPU tensors (float32, float64) are handled by the
+host library."""
 from __future__ import annotations
 
 import ctypes as C

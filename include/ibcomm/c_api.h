@@ -154,7 +154,8 @@ typedef struct {
   int dtype_out;
 } ibcomm_grad_tensor;
 /* On the current device, only enqueued.  `work`: IBCOMM_NORM_WORK doubles of device memory.  `norm` (float32, or float64
- * with norm_dtype 1) and `sum` (the sum of squares or the maximum, float64) are device memory and may be null.  With
+ * with norm_dtype 1) and `sum` (the sum of squares or the maximum, float64) are device memory and may be null.  `work` is not
+ * used by two calls at a time.  With
  * `sums` not null its num_sums values, the ranks' sums, are joined instead of the tensors' own. */
 #define IBCOMM_NORM_WORK 2048
 int ibcomm_grad_norm(const ibcomm_grad_tensor* tensors, int count, int power, const double* sums, int num_sums, double* work,
@@ -171,7 +172,9 @@ int ibcomm_scale_grads_host(const ibcomm_grad_tensor* tensors, int count, double
 int ibcomm_embedding(const void* tokens, int tokens_dtype, size_t num_tokens, const void* weight, int weight_dtype, size_t rows,
                      size_t width, void* out, int out_dtype, double scale, void* stream);
 /* out[v] = cast((accumulate ? out[v] : 0) + scale * sum of grad[t] over the t with tokens[t] == v, v != padding_row), summed in
- * float32 in the order of t.  With accumulate only rows that tokens name are touched.  padding_row -1 = none. */
+ * float32 in the order of t.  With accumulate only rows that tokens name are touched, and in float32 tables subnormal numbers
+ * are added as zero.  padding_row -1 = none.  `work`: as many bytes as ibcomm_embedding_grad_work tells, on a boundary of 256
+ * bytes; not used by two calls at a time.  No tensor that is written shares memory with another of the call. */
 int ibcomm_embedding_grad_work(size_t num_tokens, size_t rows, size_t width, size_t* bytes);
 int ibcomm_embedding_grad(const void* tokens, int tokens_dtype, size_t num_tokens, const void* grad, int grad_dtype, void* out,
                           int out_dtype, size_t rows, size_t width, int64_t padding_row, double scale, int accumulate, void* work,
