@@ -90,6 +90,11 @@ __device__ __forceinline__ SumOf<P> JoinValues(SumOf<P> sum, const A* a) {
       }
       s += t;
       if (s > 0x1p-60f && s < 0x1p126f) return sum + static_cast<double>(s);
+      // Nothing but zeros, as in the rows of an embedding that no token named.
+      unsigned any = 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) any |= __float_as_uint(a[e]);
+      if ((any & 0x7fffffffu) == 0) return sum;
     }
 #pragma unroll
     for (int e = 0; e < kN; ++e) sum = fma(static_cast<double>(a[e]), static_cast<double>(a[e]), sum);
