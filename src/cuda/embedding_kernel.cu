@@ -483,15 +483,18 @@ struct SumParams {
 // of 57), else one by one.  Rows come through a ring in shared memory, 4 KiB per
 // warp and 128 KiB per SM; in registers the same bytes left room for three blocks
 // per SM instead of four, and 131072 fp32 rows of 1024 took 180 us instead of 130.
-template <typename TG, typename TO, bool kVector>
+// kOld: 16-bit tables that are added to; what a row holds comes with the gradient of
+// the token that completes it.
+template <typename TG, typename TO, bool kVector, bool kOld>
 struct Slice {
   static constexpr int kCols = 8;
   static constexpr int kPer = !kVector ? 1 : sizeof(TG) == 2 && sizeof(TO) == 2 ? 8 : 4;  // adjacent columns
   static constexpr int kVecs = kCols / kPer;
-  static constexpr int kVecBytes = kPer * static_cast<int>(sizeof(TG));
   static constexpr int kRowBytes = 32 * kCols * static_cast<int>(sizeof(TG));
-  static constexpr int kSlotBytes = kRowBytes + (kVector ? 0 : 16);
-  static constexpr int kSlots = 4096 / kRowBytes;  // rows on their way to a warp
+  static constexpr int kGradBytes = kRowBytes + (kVector ? 0 : 16);
+  static constexpr int kOldBytes = !kOld ? 0 : 32 * kCols * static_cast<int>(sizeof(TO)) + (kVector ? 0 : 16);
+  static constexpr int kSlotBytes = kGradBytes + kOldBytes;
+  static constexpr int kSlots = kOld ? 4 : 4096 / kRowBytes;  // rows on their way to a warp
   static constexpr int kRing = kSumWarps * kSlots * kSlotBytes;
   uint64_t width;
   uint64_t column;  // the lane's first; the others are 32 * kPer apart
@@ -502,44 +505,49 @@ struct Slice {
   // A row into one of the warp's slots (`slot`: its start), without waiting for it.  With kVector a lane copies what it
   // reads itself.  Else the warp copies the 16-byte words of memory that hold the slice: no allocation ends inside one,
   // and a row may start at any element of one.
-  __device__ __forceinline__ void Fetch(const TG* row, unsigned slot) const {
+  template <typename T>
+  __device__ __forceinline__ void Fetch(const T* row, unsigned slot) const {
+    constexpr int kBytes = kPer * static_cast<int>(sizeof(T));
     const int lane = threadIdx.x & 31;
     if constexpr (kVector) {
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
         if (Has(v)) {
-          const TG* from = row + column + v * (32 * kPer);
-          const unsigned to = slot + (v * 32 + lane) * kVecBytes;
-          if constexpr (kVecBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+          const T* from = row + column + v * (32 * kPer);
+          const unsigned to = slot + (v * 32 + lane) * kBytes;
+          if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
           else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
         }
       }
     } else {
       const uint64_t first = column - lane, columns = min(width - first, static_cast<uint64_t>(32 * kCols));
-      const uintptr_t begin = reinterpret_cast<uintptr_t>(row + first), end = begin + columns * sizeof(TG);
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(row + first), end = begin + columns * sizeof(T);
 #pragma unroll
-      for (int v = 0; v < kRowBytes / 512 + 1; ++v) {
+      for (int v = 0; v < 32 * kCols * static_cast<int>(sizeof(T)) / 512 + 1; ++v) {
         const uintptr_t from = begin / 16 * 16 + (v * 32 + lane) * 16;
         if (from < end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (v * 32 + lane) * 16), "l"(from) : "memory");
       }
     }
   }
-  __device__ __forceinline__ void AddSlot(const TG* row, const unsigned char* slot, float* sum) const {
+  // sum += what Fetch has brought of `row`.
+  template <typename T>
+  __device__ __forceinline__ void AddSlot(const T* row, const unsigned char* slot, float* sum) const {
+    constexpr int kBytes = kPer * static_cast<int>(sizeof(T));
     const int lane = threadIdx.x & 31;
-    const unsigned char* at = slot + lane * kVecBytes;
+    const unsigned char* at = slot + lane * kBytes;
     if constexpr (!kVector) at += reinterpret_cast<uintptr_t>(row + (column - lane)) % 16;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      if constexpr (kVecBytes == 16) {
-        VecIO<TG>::Add(*reinterpret_cast<const uint4*>(at + v * 512), sum + v * kPer);
+      if constexpr (kBytes == 16) {
+        VecIO<T>::Add(*reinterpret_cast<const uint4*>(at + v * 512), sum + v * kPer);
       } else if constexpr (kPer == 4) {
         const uint2 q = *reinterpret_cast<const uint2*>(at + v * 256);
         float a[8];
-        VecIO<TG>::Load(make_uint4(q.x, q.y, 0, 0), a);
+        VecIO<T>::Load(make_uint4(q.x, q.y, 0, 0), a);
 #pragma unroll
         for (int e = 0; e < kPer; ++e) sum[v * kPer + e] += a[e];
       } else {
-        if (Has(v)) sum[v] += ToAcc<float, TG>(*reinterpret_cast<const TG*>(at + v * 32 * sizeof(TG)));
+        if (Has(v)) sum[v] += ToAcc<float, T>(*reinterpret_cast<const T*>(at + v * 32 * sizeof(T)));
       }
     }
   }
@@ -635,9 +643,9 @@ __device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint
 // written at once, those over the edges of parts are joined through shared
 // memory, those over the edges of the range through the workspace by the block
 // that comes last: always in the tokens' order.  `ring`: S::kRing bytes.
-template <typename TG, typename TO, bool kVector>
+template <typename TG, typename TO, bool kVector, bool kOld>
 __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uint32_t tile, unsigned char* ring) {
-  using S = Slice<TG, TO, kVector>;
+  using S = Slice<TG, TO, kVector, kOld>;
   constexpr int kCols = S::kCols;
   __shared__ float part[kSumWarps][2][32 * kCols];  // runs that began before the part, that go on behind it
   __shared__ uint32_t before_key[kSumWarps], first_key[kSumWarps], last_key[kSumWarps], behind_key[kSumWarps];
@@ -661,13 +669,20 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   const bool began_before = before == __shfl_sync(0xffffffffu, key, 0);
   const bool goes_on = behind == __shfl_sync(0xffffffffu, key, count > 0 ? count - 1 : 0);
   bool first = true;
+  auto table = [&](uint32_t k) { return static_cast<TO*>(p.out) + static_cast<uint64_t>(k) * p.width; };
   // The run that token j ends is complete.
-  auto flush = [&](int j) {
+  auto flush = [&](int j, const unsigned char* old) {
     const bool head = first && began_before;
     if (head || (goes_on && j == count - 1)) {
       float* mine = part[warp][head ? 0 : 1];
 #pragma unroll
       for (int e = 0; e < kCols; ++e) mine[e * 32 + lane] = sum[e];
+    } else if constexpr (kOld) {
+      TO* to = table(__shfl_sync(0xffffffffu, key, j));
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) sum[e] *= p.scale;
+      slice.AddSlot(to, old, sum);
+      slice.Store(to, sum);
     } else {
       WriteRow<TO>(p, slice, __shfl_sync(0xffffffffu, key, j), sum);
     }
@@ -689,12 +704,18 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   constexpr int kSlot = S::kSlotBytes;
   unsigned char* mine = ring + warp * (S::kSlots * kSlot);
   const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
-#pragma unroll
-  for (int u = 0; u < S::kSlots; ++u) {
-    const TG* r = row(u);
-    if (u < known) slice.Fetch(r, mine_shared + u * kSlot);
+  auto fetch = [&](int j, int u) {
+    const TG* r = row(j);
+    const uint32_t k = kOld ? __shfl_sync(0xffffffffu, key, j & 31) : 0;
+    if (j < known) {
+      slice.Fetch(r, mine_shared + u * kSlot);
+      if constexpr (kOld)
+        if (ends >> j & 1) slice.Fetch(static_cast<const TO*>(table(k)), mine_shared + u * kSlot + S::kGradBytes);
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  };
+#pragma unroll
+  for (int u = 0; u < S::kSlots; ++u) fetch(u, u);
   reaches();
   for (int j0 = 0; j0 < known; j0 += S::kSlots) {
 #pragma unroll
@@ -704,11 +725,13 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
         asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
         if constexpr (!kVector) __syncwarp();  // what the other lanes have copied
         slice.AddSlot(row(j), mine + u * kSlot, sum);
+        // With kOld the slot is needed for the flush; else the next row is sent for first.
+        if constexpr (kOld)
+          if (ends >> j & 1) flush(j, mine + u * kSlot + S::kGradBytes);
         if constexpr (!kVector) __syncwarp();  // they have read it
-        const TG* r = row(j + S::kSlots);
-        if (j + S::kSlots < known) slice.Fetch(r, mine_shared + u * kSlot);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (ends >> j & 1) flush(j);
+        fetch(j + S::kSlots, u);
+        if constexpr (!kOld)
+          if (ends >> j & 1) flush(j, nullptr);
       }
     }
   }
@@ -780,12 +803,12 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   }
 }
 
-template <typename TG, typename TO, bool kVector>
+template <typename TG, typename TO, bool kVector, bool kOld>
 __global__ void __launch_bounds__(kSumThreads, 4) SumRunsKernel(SumParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   WaitForPrevious();
   const uint32_t range = blockIdx.x / p.tiles;
-  SumRange<TG, TO, kVector>(p, range, blockIdx.x - range * p.tiles, ring);
+  SumRange<TG, TO, kVector, kOld>(p, range, blockIdx.x - range * p.tiles, ring);
 }
 
 // Few tokens: every block sorts them all, by counting for each how many come
@@ -803,7 +826,7 @@ struct SmallParams {
   uint32_t clear_rows;  // of a block
 };
 
-template <typename TG, typename TO, bool kVector>
+template <typename TG, typename TO, bool kVector, bool kOld>
 __global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ __align__(16) uint32_t keys[kSmallTokens], sorted[kSmallTokens], positions[kSmallTokens], named[kClearRows / 32];
@@ -831,7 +854,7 @@ __global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p)
     SumParams sum = p.sum;
     sum.key = sorted;
     sum.position = positions;
-    SumRange<TG, TO, kVector>(sum, 0, blockIdx.x, ring);
+    SumRange<TG, TO, kVector, kOld>(sum, 0, blockIdx.x, ring);
     return;
   }
   const uint32_t first = (blockIdx.x - p.sum.tiles) * p.clear_rows, rows = min(p.clear_rows, p.sum.rows - first);
@@ -1090,7 +1113,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
   return WithTypes(p.dtype_grad, p.dtype_out, [&](auto tg, auto to) {
     using TG = decltype(tg);
     using TO = decltype(to);
-    constexpr uint64_t kPer = dev::Slice<TG, TO, true>::kPer;
+    constexpr uint64_t kPer = dev::Slice<TG, TO, true, false>::kPer;
     auto aligned = [](const void* a, size_t bytes) { return reinterpret_cast<uintptr_t>(a) % std::min<size_t>(bytes, 16) == 0; };
     const bool vector = p.width % kPer == 0 && aligned(p.grad, kPer * sizeof(TG)) && aligned(p.out, kPer * sizeof(TO));
     const unsigned grid = static_cast<unsigned>(part.ranges * part.tiles);
@@ -1106,14 +1129,22 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
         kernel<<<static_cast<unsigned>(blocks), dev::kSumThreads, ring, stream>>>(small);
         return cudaGetLastError();
       };
-      return vector ? launch(dev::FewTokensKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::FewTokensKernel<TG, TO, false>, dev::Slice<TG, TO, false>::kRing);
+      if constexpr (sizeof(TO) == 2)
+        if (p.accumulate) return vector ? launch(dev::FewTokensKernel<TG, TO, true, true>, dev::Slice<TG, TO, true, true>::kRing)
+                                        : launch(dev::FewTokensKernel<TG, TO, false, true>, dev::Slice<TG, TO, false, true>::kRing);
+      return vector ? launch(dev::FewTokensKernel<TG, TO, true, false>, dev::Slice<TG, TO, true, false>::kRing)
+                    : launch(dev::FewTokensKernel<TG, TO, false, false>, dev::Slice<TG, TO, false, false>::kRing);
     }
     auto launch = [&](auto kernel, int ring) {
       const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));
       if (e != cudaSuccess) return e;
       return LaunchEarly(kernel, grid, dev::kSumThreads, static_cast<size_t>(ring), stream, sum);
     };
-    return vector ? launch(dev::SumRunsKernel<TG, TO, true>, dev::Slice<TG, TO, true>::kRing) : launch(dev::SumRunsKernel<TG, TO, false>, dev::Slice<TG, TO, false>::kRing);
+    if constexpr (sizeof(TO) == 2)
+      if (p.accumulate) return vector ? launch(dev::SumRunsKernel<TG, TO, true, true>, dev::Slice<TG, TO, true, true>::kRing)
+                                      : launch(dev::SumRunsKernel<TG, TO, false, true>, dev::Slice<TG, TO, false, true>::kRing);
+    return vector ? launch(dev::SumRunsKernel<TG, TO, true, false>, dev::Slice<TG, TO, true, false>::kRing)
+                  : launch(dev::SumRunsKernel<TG, TO, false, false>, dev::Slice<TG, TO, false, false>::kRing);
   });
 }
 
