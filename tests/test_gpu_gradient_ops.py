@@ -415,6 +415,11 @@ def test_gradient_widths_types_and_alignment(width, table, rows_type):
         want, bound = grad_in_64_bits(t, g, rows, 1.0)
         ar.ops.embedding_grad(t, g, out=out)
         within(out, want, bound + half(table) * want.abs() + least(table))
+        old = values((rows, width), table, 9)
+        out.copy_(old)
+        ar.ops.embedding_grad(t, g, out=out, accumulate=True)
+        want = want + old.double()
+        within(out, want, bound + U * (old.double().abs() + want.abs()) + half(table) * want.abs() + least(table))
         assert torch.all(guard[:offsets[1]] == 7) and torch.all(guard[offsets[1] + rows * width:] == 7)
 
 
