@@ -1,7 +1,7 @@
 """Embedding lookup with scaling, and the gradient of its table.
 
-The gradient is summed by sorted tokens: every row of the table is written once, by one warp per slice of its columns,
-in float32 and in the order of the tokens.  It is the same for the same inputs, whatever ran beside it, so ranks that
+The gradient is summed by sorted tokens: every row of the table is written once, the sum of its tokens' rows in float32,
+in parts that are joined in the tokens' order.  It is the same for the same inputs, whatever ran beside it, so ranks that
 hold replicas agree; and it can be added straight into a gradient bucket, where only the rows that tokens name are
 touched.  Tokens outside of the table give a row of zeros and no gradient: padded places (-1), or the tokens of another
 rank's part of a table that is split by rows (look up ``tokens - first_row`` and allreduce the rows)."""

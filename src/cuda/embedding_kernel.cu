@@ -812,10 +812,14 @@ __global__ void __launch_bounds__(kSumThreads, 4) SumRunsKernel(SumParams p) {
 }
 
 // Few tokens: every block sorts them all, by counting for each how many come
-// before it, and adds in its slice of the columns.  The blocks behind clear rows
-// that no token names.  One launch: 33 rows of 768 bf16 3.3 us on the device
-// against 11 with the kernels above, 256 rows 11.1 against 11.2, where it ends.
+// before it, and adds the runs that begin in its part of the list, in its slice
+// of the columns.  The blocks behind clear rows that no token names.  One launch:
+// 33 rows of 768 bf16 3.3 us on the device against 11 with the kernels above, 256
+// rows 5.7 against 11.1 (11.1 too with one part: an SM hands its additions to the
+// memory one sector at a time).  More tokens than threads are not taken: a block
+// would count for n * n / 256 pairs.
 constexpr uint32_t kSmallTokens = kSumThreads;
+constexpr uint32_t kPartTokens = 32;  // of a block: four per warp
 constexpr uint32_t kClearRows = 8192;  // of a block, at most
 
 struct SmallParams {
@@ -823,13 +827,14 @@ struct SmallParams {
   const void* tokens;
   int tokens_are_64;
   int64_t padding;
+  uint32_t parts;       // of the list, a block per part and slice
   uint32_t clear_rows;  // of a block
 };
 
 template <typename TG, typename TO, bool kVector, bool kOld>
 __global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p) {
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ __align__(16) uint32_t keys[kSmallTokens], sorted[kSmallTokens], positions[kSmallTokens], named[kClearRows / 32];
+  __shared__ __align__(16) uint32_t keys[kSmallTokens], sorted[kSmallTokens], positions[kSmallTokens], named[kClearRows / 32], bounds[2];
   const uint32_t t = threadIdx.x, n = p.sum.n;
   SortParams of{};
   of.tokens = p.tokens;
@@ -837,7 +842,7 @@ __global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p)
   of.rows = p.sum.rows;
   of.padding = p.padding;
   const uint32_t key = t < n ? KeyOf(of, t) : kNoKey;
-  if (blockIdx.x < p.sum.tiles) {
+  if (blockIdx.x < p.sum.tiles * p.parts) {
     keys[t] = key;
     __syncthreads();
     uint32_t rank = 0;
@@ -850,14 +855,24 @@ __global__ void __launch_bounds__(kSumThreads, 4) FewTokensKernel(SmallParams p)
       sorted[rank] = key;
       positions[rank] = t;
     }
+    if (t < 2) bounds[t] = n;
+    __syncthreads();
+    // The block's share: from the first run that begins in its part of the list to the first that begins behind it.
+    const uint32_t part = blockIdx.x / p.sum.tiles, lo = part * n / p.parts, hi = (part + 1) * n / p.parts;
+    if (t < n && (t == 0 || sorted[t] != sorted[t - 1])) {
+      if (t >= lo) atomicMin(&bounds[0], t);
+      if (t >= hi) atomicMin(&bounds[1], t);
+    }
     __syncthreads();
     SumParams sum = p.sum;
-    sum.key = sorted;
-    sum.position = positions;
-    SumRange<TG, TO, kVector, kOld>(sum, 0, blockIdx.x, ring);
+    sum.key = sorted + bounds[0];
+    sum.position = positions + bounds[0];
+    sum.n = bounds[1] - bounds[0];
+    sum.per_warp = (sum.n + kSumWarps - 1) / kSumWarps;
+    if (sum.n > 0) SumRange<TG, TO, kVector, kOld>(sum, 0, blockIdx.x - part * p.sum.tiles, ring);
     return;
   }
-  const uint32_t first = (blockIdx.x - p.sum.tiles) * p.clear_rows, rows = min(p.clear_rows, p.sum.rows - first);
+  const uint32_t first = (blockIdx.x - p.sum.tiles * p.parts) * p.clear_rows, rows = min(p.clear_rows, p.sum.rows - first);
   for (uint32_t i = t; i < kClearRows / 32; i += kSumThreads) named[i] = 0;
   __syncthreads();
   if (key >= first && key - first < rows) atomicOr(&named[(key - first) / 32], 1u << (key - first) % 32);
@@ -1118,10 +1133,10 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     const bool vector = p.width % kPer == 0 && aligned(p.grad, kPer * sizeof(TG)) && aligned(p.out, kPer * sizeof(TO));
     const unsigned grid = static_cast<unsigned>(part.ranges * part.tiles);
     if (few) {
-      dev::SmallParams small{sum, p.tokens, p.tokens_are_64, p.padding, 0};
+      dev::SmallParams small{sum, p.tokens, p.tokens_are_64, p.padding, (sum.n + dev::kPartTokens - 1) / dev::kPartTokens, 0};
       const uint64_t row = p.width * sizeof(TO);
       small.clear_rows = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(kFewClearBytes / row, 1), dev::kClearRows));
-      const uint64_t blocks = part.tiles + (p.accumulate ? 0 : (p.rows + small.clear_rows - 1) / small.clear_rows);
+      const uint64_t blocks = part.tiles * small.parts + (p.accumulate ? 0 : (p.rows + small.clear_rows - 1) / small.clear_rows);
       if (blocks > 0x7fffffffull) return cudaErrorInvalidValue;
       auto launch = [&](auto kernel, int ring) {
         const cudaError_t e = AllowSharedMemory(kernel, static_cast<size_t>(ring));

@@ -380,7 +380,7 @@ def test_lookup_of_tokens_of_any_shape():
 
 
 # Around a chunk of tokens, a sort's block, and several blocks; rows from one to more than one digit of the sort.
-@pytest.mark.parametrize("n,rows", [(1, 1), (2, 1), (31, 3), (32, 1000), (33, 2), (64, 64), (100, 5000), (257, 1), (500, 1), (1000, 1023), (1000, 1024),
+@pytest.mark.parametrize("n,rows", [(1, 1), (2, 1), (31, 3), (32, 1000), (33, 2), (64, 64), (100, 5000), (200, 1), (255, 3), (256, 40), (257, 1), (500, 1), (1000, 1023), (1000, 1024),
                                     (2047, 100), (2049, 200000), (5000, 7), (20000, 300), (70000, 1 << 20)])
 @pytest.mark.parametrize("table,rows_type", [(F32, BF16), (F32, F32), (BF16, BF16), (F16, F32)])
 def test_gradient_of_the_table(table, rows_type, n, rows):
@@ -641,6 +641,40 @@ def test_step_in_a_graph():
     want = step()
     for a, b in zip(kept, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_bucket_step_in_a_graph(dtype):
+    # Lookup, backward pass into the bucket, allreduce, clipping: nothing of it is read back.
+    buckets = ar.GradientBuckets([(50, 24), (24,)], dtype=dtype, comm=ar.Communicator(1, 0))
+    w, h = torch.nn.Parameter(values((50, 24), dtype, 1)), torch.nn.Parameter(values((24,), dtype, 2))
+    buckets.attach([w, h])
+    t = tokens_of(500, 50, 3)
+
+    def step():
+        buckets.zero_()
+        (buckets.embedding(0, t, w, scale=0.25) * h).sum().backward()
+        buckets.allreduce()
+        return buckets.clip_grad_norm(1.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = step()
+    t.copy_(tokens_of(500, 50, 4))
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [norm.clone(), buckets.flat[0].clone()]
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want) and torch.equal(got[1], buckets.flat[0])
+    inside = ((t >= 0) & (t < 50)).sum().item()
+    assert 0 < inside < 500 and torch.isfinite(want)
 
 
 IN_GRAPH = """
