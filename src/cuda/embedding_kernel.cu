@@ -615,25 +615,39 @@ __device__ __forceinline__ void WriteRow(const SumParams& p, const S& slice, uin
   }
 }
 
-// The first and last range of the run of `k` that goes over an edge of `range`.
+// The first and last range of the run of `k` that goes over an edge of `range`: a
+// look at the 32 edges next to it, and a search in steps of a 32nd where the run
+// goes over all of them.
 __device__ __forceinline__ void RangesOfRun(const SumParams& p, uint32_t k, uint32_t range, uint32_t* first, uint32_t* last) {
   const uint32_t lane = threadIdx.x & 31, per = p.per_warp * kSumWarps;
-  // Whether the run goes over the edge between range b - 1 and range b.
-  auto crosses = [&](uint32_t b) { return b >= 1 && b < p.ranges && p.key[b * per - 1] == k && p.key[b * per] == k; };
-  uint32_t c = range;
-  for (;;) {
-    const unsigned m = __ballot_sync(0xffffffffu, c >= lane && crosses(c - lane));
-    const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-    c -= run;
-    if (run < 32) break;
+  // Whether the run goes over edge b, which is that between range b - 1 and range b, if it goes over the next one, or the one before.
+  auto from_left = [&](uint32_t b) { return b >= 1 && p.key[b * per - 1] == k; };
+  auto to_right = [&](uint32_t b) { return b < p.ranges && p.key[b * per] == k; };
+  const bool over_left = from_left(range) && to_right(range);
+  unsigned m = __ballot_sync(0xffffffffu, over_left && range >= lane && from_left(range - lane));
+  uint32_t c = range - (m == 0xffffffffu ? 32 : __ffs(~m) - 1);  // the run goes over the edges c + 1 to range
+  if (m == 0xffffffffu) {
+    uint32_t lo = 0, hi = c + 1;  // not over edge lo, over edge hi
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo + 31) / 32, b = lo + step * (lane + 1);
+      const int f = __ffs(__ballot_sync(0xffffffffu, b >= hi || from_left(b))) - 1;
+      hi = min(hi, lo + step * (f + 1));
+      lo += step * f;
+    }
+    c = hi - 1;
   }
   *first = c;
-  c = range;
-  for (;;) {
-    const unsigned m = __ballot_sync(0xffffffffu, crosses(c + 1 + lane));
-    const int run = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-    c += run;
-    if (run < 32) break;
+  m = __ballot_sync(0xffffffffu, range + 1 < p.ranges && from_left(range + 1) && to_right(range + 1 + lane));
+  c = range + (m == 0xffffffffu ? 32 : __ffs(~m) - 1);  // over the edges range + 1 to c
+  if (m == 0xffffffffu) {
+    uint32_t lo = c, hi = p.ranges;  // over edge lo, not over edge hi
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo + 31) / 32, b = lo + step * (lane + 1);
+      const int f = __ffs(__ballot_sync(0xffffffffu, b >= hi || !to_right(b))) - 1;
+      hi = min(hi, lo + step * (f + 1));
+      lo += step * f;
+    }
+    c = lo;
   }
   *last = c;
 }

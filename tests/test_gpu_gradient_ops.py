@@ -423,7 +423,7 @@ def test_gradient_widths_types_and_alignment(width, table, rows_type):
         assert torch.all(guard[:offsets[1]] == 7) and torch.all(guard[offsets[1] + rows * width:] == 7)
 
 
-@pytest.mark.parametrize("n", [1, 40, 300, 9000, 100000])
+@pytest.mark.parametrize("n", [1, 40, 300, 9000, 100000, 600000])
 def test_all_tokens_the_same_or_none(n):
     g = values((n, 72), F32, n)
     for token, rows in ((0, 1), (6, 9), (8, 9), (-1, 9), (9, 9), (-2 ** 31, 9), (2 ** 31 - 1, 9)):
