@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kClearThreads) ClearKernel(unsigned char* out,
 // -------------------------------------------------------------------- sums
 constexpr int kSumWarps = 8;
 constexpr int kSumThreads = 32 * kSumWarps;
-constexpr int kMostWarpTokens = 16;  // with 8 or 32, 16384 rows of 4096 take 82 or 77 us instead of 75
+constexpr int kWarpTokens = 16;  // with 8 or 32, 16384 rows of 4096 take 82 or 77 us instead of 75
 constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct SumParams {
@@ -465,7 +465,7 @@ struct SumParams {
   const uint32_t* position;
   uint32_t n;
   uint32_t rows;
-  uint32_t per_warp;  // tokens, 32 at most
+  uint32_t per_warp;  // tokens: 32 at most, or a multiple of 32
   uint32_t ranges;    // of kSumWarps * per_warp tokens
   uint32_t tiles;     // slices of the columns
   const void* grad;
@@ -668,94 +668,112 @@ __device__ __forceinline__ void SumRange(const SumParams& p, uint32_t range, uin
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const uint32_t i0 = (range * kSumWarps + warp) * p.per_warp;
   const int count = i0 < p.n ? static_cast<int>(min(p.per_warp, p.n - i0)) : 0;
-  const uint32_t key = lane < count ? p.key[i0 + lane] : kNoKey;
-  const uint32_t position = lane < count ? p.position[i0 + lane] : 0;
   const uint32_t before = count > 0 && i0 > 0 ? p.key[i0 - 1] : kNoKey;
+  const uint32_t last = count > 0 ? p.key[i0 + count - 1] : kNoKey;
   const uint32_t behind = count > 0 && i0 + count < p.n ? p.key[i0 + count] : kNoKey;
-  const int known = __popc(__ballot_sync(0xffffffffu, key < p.rows));  // tokens without a row come last
   const TG* grad = static_cast<const TG*>(p.grad);
   float sum[kCols];
 #pragma unroll
   for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
-  // The tokens that end a run, and whether the first and the last run go over the part's edges.
-  const uint32_t next = __shfl_down_sync(0xffffffffu, key, 1);
-  const unsigned ends = __ballot_sync(0xffffffffu, lane < known && (lane == count - 1 || key != next));
-  const bool began_before = before == __shfl_sync(0xffffffffu, key, 0);
-  const bool goes_on = behind == __shfl_sync(0xffffffffu, key, count > 0 ? count - 1 : 0);
-  bool first = true;
+  // 32 tokens of the part, a lane holds one.
+  struct Held {
+    uint32_t key, position;
+    int known;      // those with a row, which come first
+    unsigned ends;  // those that end a run, or the part
+  };
+  auto hold = [&](int at) {
+    Held h;
+    const int n = min(max(count - at, 0), 32);
+    h.key = lane < n ? p.key[i0 + at + lane] : kNoKey;
+    h.position = lane < n ? p.position[i0 + at + lane] : 0;
+    const uint32_t after = n > 0 && i0 + at + n < p.n ? p.key[i0 + at + n] : kNoKey;
+    uint32_t next = __shfl_down_sync(0xffffffffu, h.key, 1);
+    if (lane == n - 1) next = at + n == count ? kNoKey : after;
+    h.known = __popc(__ballot_sync(0xffffffffu, h.key < p.rows));
+    h.ends = __ballot_sync(0xffffffffu, lane < h.known && h.key != next);
+    return h;
+  };
+  Held held = hold(0), ahead = hold(32);
+  // Whether the first and the last run go over the part's edges.
+  const uint32_t begin_key = __shfl_sync(0xffffffffu, held.key, 0);
+  const bool began_before = begin_key < p.rows && before == begin_key;
+  const bool goes_on = last < p.rows && behind == last;
+  bool first = true;  // no run of the part has ended
   auto table = [&](uint32_t k) { return static_cast<TO*>(p.out) + static_cast<uint64_t>(k) * p.width; };
-  // The run that token j ends is complete.
-  auto flush = [&](int j, const unsigned char* old) {
+  // The run that token j of the part, of row k, ends is complete.
+  auto flush = [&](int j, uint32_t k, const unsigned char* old) {
     const bool head = first && began_before;
     if (head || (goes_on && j == count - 1)) {
       float* mine = part[warp][head ? 0 : 1];
 #pragma unroll
       for (int e = 0; e < kCols; ++e) mine[e * 32 + lane] = sum[e];
     } else if constexpr (kOld) {
-      TO* to = table(__shfl_sync(0xffffffffu, key, j));
+      TO* to = table(k);
 #pragma unroll
       for (int e = 0; e < kCols; ++e) sum[e] *= p.scale;
       slice.AddSlot(to, old, sum);
       slice.Store(to, sum);
     } else {
-      WriteRow<TO>(p, slice, __shfl_sync(0xffffffffu, key, j), sum);
+      WriteRow<TO>(p, slice, k, sum);
     }
     first = false;
 #pragma unroll
     for (int e = 0; e < kCols; ++e) sum[e] = 0.f;
   };
-  auto row = [&](int j) { return grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, position, j & 31)) * p.width; };
+  auto row = [&](const Held& h, int j) { return grad + static_cast<uint64_t>(__shfl_sync(0xffffffffu, h.position, j)) * p.width; };
   // How far the runs over the range's edges reach, looked up while the first rows are on their way.
   auto reach = [&](int side, uint32_t k) {
     uint32_t a, b;
     RangesOfRun(p, k, range, &a, &b);
     if (lane == 0) run_first[side] = a, run_last[side] = b;
   };
-  auto reaches = [&] {
-    if (warp == 0 && began_before && known > 0) reach(0, __shfl_sync(0xffffffffu, key, 0));
-    if (warp == kSumWarps - 1 && goes_on && known == count && count > 0) reach(1, __shfl_sync(0xffffffffu, key, count - 1));
-  };
   constexpr int kSlot = S::kSlotBytes;
   unsigned char* mine = ring + warp * (S::kSlots * kSlot);
   const unsigned mine_shared = static_cast<unsigned>(__cvta_generic_to_shared(mine));
-  auto fetch = [&](int j, int u) {
-    const TG* r = row(j);
-    const uint32_t k = kOld ? __shfl_sync(0xffffffffu, key, j & 31) : 0;
-    if (j < known) {
+  auto fetch = [&](const Held& h, int j, int u) {
+    const TG* r = row(h, j);
+    const uint32_t k = kOld ? __shfl_sync(0xffffffffu, h.key, j) : 0;
+    if (j < h.known) {
       slice.Fetch(r, mine_shared + u * kSlot);
       if constexpr (kOld)
-        if (ends >> j & 1) slice.Fetch(static_cast<const TO*>(table(k)), mine_shared + u * kSlot + S::kGradBytes);
+        if (h.ends >> j & 1) slice.Fetch(static_cast<const TO*>(table(k)), mine_shared + u * kSlot + S::kGradBytes);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int u = 0; u < S::kSlots; ++u) fetch(u, u);
-  reaches();
-  for (int j0 = 0; j0 < known; j0 += S::kSlots) {
+  for (int u = 0; u < S::kSlots; ++u) fetch(held, u, u);
+  if (warp == 0 && began_before) reach(0, begin_key);
+  if (warp == kSumWarps - 1 && goes_on) reach(1, last);
+  for (int at = 0; at < count; at += 32) {
+    for (int j0 = 0; j0 < held.known; j0 += S::kSlots) {
 #pragma unroll
-    for (int u = 0; u < S::kSlots; ++u) {
-      const int j = j0 + u;
-      if (j < known) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
-        if constexpr (!kVector) __syncwarp();  // what the other lanes have copied
-        slice.AddSlot(row(j), mine + u * kSlot, sum);
-        // With kOld the slot is needed for the flush; else the next row is sent for first.
-        if constexpr (kOld)
-          if (ends >> j & 1) flush(j, mine + u * kSlot + S::kGradBytes);
-        if constexpr (!kVector) __syncwarp();  // they have read it
-        fetch(j + S::kSlots, u);
-        if constexpr (!kOld)
-          if (ends >> j & 1) flush(j, nullptr);
+      for (int u = 0; u < S::kSlots; ++u) {
+        const int j = j0 + u;
+        if (j < held.known) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
+          if constexpr (!kVector) __syncwarp();  // what the other lanes have copied
+          slice.AddSlot(row(held, j), mine + u * kSlot, sum);
+          // With kOld the slot is needed for the flush; else the next row is sent for first.
+          if constexpr (kOld)
+            if (held.ends >> j & 1) flush(at + j, __shfl_sync(0xffffffffu, held.key, j), mine + u * kSlot + S::kGradBytes);
+          if constexpr (!kVector) __syncwarp();  // they have read it
+          if (j + S::kSlots < 32) fetch(held, j + S::kSlots, u);
+          else fetch(ahead, j + S::kSlots - 32, u);
+          if constexpr (!kOld)
+            if (held.ends >> j & 1) flush(at + j, __shfl_sync(0xffffffffu, held.key, j), nullptr);
+        }
       }
     }
+    held = ahead;
+    ahead = hold(at + 64);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (lane == 0) {
     before_key[warp] = before;
-    first_key[warp] = key;
+    first_key[warp] = begin_key;
+    last_key[warp] = last;
     behind_key[warp] = behind;
   }
-  if (lane == (count > 0 ? count - 1 : 0)) last_key[warp] = key;
   __syncthreads();
   // Runs over the edges of parts.
   const bool from_before = first_key[0] < p.rows && before_key[0] == first_key[0];
@@ -1041,15 +1059,19 @@ struct SumShape {
   uint32_t per_warp;
   uint64_t ranges, tiles;
 };
-SumShape SumShapeOf(uint64_t n, uint64_t width) {
+SumShape SumShapeOf(uint64_t n, uint64_t rows, uint64_t width) {
   SumShape s;
-  s.per_warp = n > dev::kSmallTokens ? dev::kMostWarpTokens : static_cast<uint32_t>((n + dev::kSumWarps - 1) / dev::kSumWarps);
+  s.per_warp = n > dev::kSmallTokens ? dev::kWarpTokens : static_cast<uint32_t>((n + dev::kSumWarps - 1) / dev::kSumWarps);
   s.tiles = (width + 255) / 256;
   auto ranges = [&] { return (n + s.per_warp * dev::kSumWarps - 1) / (s.per_warp * dev::kSumWarps); };
   // Shorter parts where the blocks would not fill the GPU twice (148 SMs): their lengths are then what counts, not the runs over
   // their edges.  600 tokens of 768 13.5 -> 9.3 us, 8192 18.8 -> 17.9; 600 of 4096, skewed, 11.7 -> 12.7.
   if (n > dev::kSmallTokens)
     while (s.per_warp > 4 && ranges() * s.tiles < 2 * 148) s.per_warp /= 2;
+  // Longer ones where the runs are long, at least on average, so that every range has one over each edge; as long as the blocks
+  // fill the GPU (four per SM).
+  if (n / std::max<uint64_t>(rows, 1) >= 8)
+    while (s.per_warp < 128 && ranges() * s.tiles >= 2 * 4 * 148) s.per_warp *= 2;
   s.ranges = n > 0 ? ranges() : 0;
   return s;
 }
@@ -1057,7 +1079,7 @@ SumShape SumShapeOf(uint64_t n, uint64_t width) {
 size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
   if (n <= dev::kSmallTokens) return 0;
   const SortShape s = ShapeOf(n, rows);
-  const SumShape sum = SumShapeOf(n, width);
+  const SumShape sum = SumShapeOf(n, rows, width);
   return 4 * Padded(n * 4) + Padded(static_cast<size_t>(s.blocks) << s.bits << 2) + Padded(sum.ranges * sum.tiles * 4) + 2 * sum.ranges * width * 4;
 }
 
@@ -1123,7 +1145,7 @@ cudaError_t LaunchEmbeddingGrad(const EmbeddingGradParams& p, cudaStream_t strea
     return cudaGetLastError();
   }
   if (p.work_bytes < EmbeddingGradWorkBytes(p.num_tokens, p.rows, p.width)) return cudaErrorInvalidValue;
-  const SumShape part = SumShapeOf(p.num_tokens, p.width);
+  const SumShape part = SumShapeOf(p.num_tokens, p.rows, p.width);
   if (part.ranges * part.tiles > 0x7fffffffull) return cudaErrorInvalidValue;
   dev::SumParams sum{};
   sum.n = static_cast<uint32_t>(p.num_tokens);
