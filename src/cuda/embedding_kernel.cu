@@ -1068,10 +1068,11 @@ SumShape SumShapeOf(uint64_t n, uint64_t rows, uint64_t width) {
   // their edges.  600 tokens of 768 13.5 -> 9.3 us, 8192 18.8 -> 17.9; 600 of 4096, skewed, 11.7 -> 12.7.
   if (n > dev::kSmallTokens)
     while (s.per_warp > 4 && ranges() * s.tiles < 2 * 148) s.per_warp /= 2;
-  // Longer ones where the runs are long, at least on average, so that every range has one over each edge; as long as the blocks
-  // fill the GPU (four per SM).
+  // Longer ones where the runs are long, at least on average, so that every range has one over each edge, as long as there are
+  // two blocks per SM; 128 tokens only where there are eight.  Rows of bf16, 2 rows in the table: 32768 of 1024 33.7 us with 16
+  // or 32, 27.2 with 64; 131072 of 1024 74.0 with 64, 74.8 with 128; 1 M of 512 527 with 16, 274 with 64, 260 with 128.
   if (n / std::max<uint64_t>(rows, 1) >= 8)
-    while (s.per_warp < 128 && ranges() * s.tiles >= 2 * 4 * 148) s.per_warp *= 2;
+    while (s.per_warp < 128 && ranges() * s.tiles >= (s.per_warp < 64 ? 4 : 16) * 148) s.per_warp *= 2;
   s.ranges = n > 0 ? ranges() : 0;
   return s;
 }
