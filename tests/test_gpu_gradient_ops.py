@@ -404,6 +404,21 @@ def test_gradient_of_the_table(table, rows_type, n, rows):
     within(into[named], want, bound + (U * (old[named].double().abs() + want.abs()) + half(table) * want.abs()) + least(table))
 
 
+@pytest.mark.parametrize("n,width", [(200003, 264), (700001, 264), (300001, 33)])
+@pytest.mark.parametrize("table,rows_type", [(F32, BF16), (F32, F32), (BF16, BF16)])
+def test_gradient_of_few_rows(table, rows_type, n, width):
+    # Long runs: a warp's part of the list is longer than the 32 tokens that its lanes hold.
+    rows = 40
+    t, g = tokens_of(n, rows, n, torch.int32), values((n, width), rows_type, width)
+    want, bound = grad_in_64_bits(t, g, rows, 0.5)
+    within(ar.ops.embedding_grad(t, g, num_rows=rows, dtype=table, scale=0.5), want, bound + half(table) * want.abs())
+    old = values((rows, width), table, 7)
+    into = old.clone()
+    ar.ops.embedding_grad(t, g, out=into, accumulate=True, scale=0.5)
+    want = want + old.double()
+    within(into, want, bound + U * (old.double().abs() + want.abs()) + half(table) * want.abs())
+
+
 @pytest.mark.parametrize("table,rows_type", TYPES)
 @pytest.mark.parametrize("width", [1, 3, 4, 8, 100, 129, 255, 256, 1000, 2056])
 def test_gradient_widths_types_and_alignment(width, table, rows_type):
