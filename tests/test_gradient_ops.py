@@ -1,7 +1,6 @@
 """The gradient norm, clipping and the embedding without a GPU: the host path of the first two, and what the entry points
 refuse before anything is launched."""
 import ctypes as C
-
 import math
 import subprocess
 import sys
