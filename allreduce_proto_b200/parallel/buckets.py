@@ -64,6 +64,9 @@ class GradientBuckets:
         self.plan = plan_buckets(numels, esize, bucket_bytes)
         self.flat: list[torch.Tensor] = []
         self.views: list[torch.Tensor] = [None] * len(self.shapes)  # type: ignore[list-item]
+        # What a bucket holds of gradients, without the places in between and behind: tensors that follow one another make one run.
+        self._runs: list[torch.Tensor] = []
+        self._own_runs: list[torch.Tensor] = []  # inside this rank's blocks
         for idxs in self.plan:
             offs, total = [], 0
             for i in idxs:
@@ -81,6 +84,20 @@ class GradientBuckets:
             self.flat.append(buf)
             for i, o in zip(idxs, offs):
                 self.views[i] = buf[o:o + numels[i]].view(self.shapes[i])
+            runs: list[list[int]] = []
+            for i, o in zip(idxs, offs):
+                if runs and runs[-1][1] == o:
+                    runs[-1][1] += numels[i]
+                elif numels[i] > 0:
+                    runs.append([o, o + numels[i]])
+            self._runs += [buf[a:b] for a, b in runs]
+            if shardable:
+                m = total // (1 if comm is None else comm.world_size)
+                lo = 0 if comm is None else comm.rank * m
+                self._own_runs += [buf[max(a, lo):min(b, lo + m)] for a, b in runs if max(a, lo) < min(b, lo + m)]
+        # The norm takes its device and type from a tensor of no elements where there is no other.
+        self._runs = self._runs or [b[:0] for b in self.flat[:1]]
+        self._own_runs = self._own_runs or [b[:0] for b in self.flat[:1]]
 
     @property
     def num_buckets(self) -> int:
@@ -151,18 +168,25 @@ class GradientBuckets:
             self.comm.all_gather(shard, buf, algo=algo, sync=sync)
 
     # ----------------------------------------------------- norm and clipping
+    def _gradients(self, sharded: bool) -> list[torch.Tensor]:
+        # Not the whole buckets: a norm that is not a number makes NaN of all that is scaled, and what lies between the
+        # gradients is written by nobody else, so it would stay NaN for every later step.
+        if sharded and not self.shardable:
+            raise ValueError("construct GradientBuckets with shardable=True")
+        return self._own_runs if sharded else self._runs
+
     def grad_norm(self, *, norm_type: float = 2.0, sharded: bool = False) -> torch.Tensor:
         """The norm of all gradients (call it after :meth:`allreduce` or :meth:`finish`).
 
         ``sharded``: after :meth:`reduce_scatter`, from this rank's blocks and one value of every other rank's."""
         from ..ops.gradients import grad_norm
-        return grad_norm(self.shards() if sharded else self.flat, norm_type=norm_type, comm=self.comm if sharded else None)
+        return grad_norm(self._gradients(sharded), norm_type=norm_type, comm=self.comm if sharded else None)
 
     def clip_grad_norm(self, max_norm: float, *, norm_type: float = 2.0, sharded: bool = False) -> torch.Tensor:
         """Scales the gradients (``sharded``: this rank's blocks) so that their norm is at most ``max_norm``, in
         place, and returns the norm they had; see :func:`allreduce_proto_b200.ops.clip_grad_norm`."""
         from ..ops.gradients import clip_grad_norm
-        return clip_grad_norm(self.shards() if sharded else self.flat, max_norm, norm_type=norm_type,
+        return clip_grad_norm(self._gradients(sharded), max_norm, norm_type=norm_type,
                               comm=self.comm if sharded else None)
 
     # ------------------------------------------------------------- embedding

@@ -787,3 +787,21 @@ def test_what_is_refused_on_the_gpu():
     assert code_of(lambda: ar.ops.embedding_grad(t, g, out=torch.ones(8, 4, device="cuda").t())) == ar.INVALID_ARGUMENT
     torch.cuda.synchronize()
     assert torch.all(x == 1) and torch.all(w == 1)
+
+
+@pytest.mark.parametrize("sharded", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_buckets_recover_from_a_step_that_is_not_a_number(dtype, sharded):
+    # Every tensor leaves places up to the next 16 bytes, which only zero_() writes.
+    shapes = [(5,), (7,), (3, 33)]
+    buckets = ar.GradientBuckets(shapes, dtype=dtype, shardable=True)
+    grads = [values(s, dtype, i) for i, s in enumerate(shapes)]
+    buckets.load([torch.full_like(grads[0], math.nan)] + grads[1:])
+    assert math.isnan(buckets.clip_grad_norm(1.0, sharded=sharded)) and torch.isnan(buckets.views[2]).all()
+    buckets.load(grads)
+    want = norm_of(grads, 2)
+    within(buckets.grad_norm(), want, 5.5 * U * want.item())
+    within(buckets.clip_grad_norm(0.5, sharded=sharded), want, 5.5 * U * want.item())
+    for v, g in zip(buckets.views, grads):
+        w = g.double() * (0.5 / (want.item() + 1e-6))
+        within(v, w, (6.5 * U + half(dtype)) * w.abs())

@@ -81,6 +81,31 @@ def test_buckets_on_the_host():
         torch.testing.assert_close(v.double(), g.double() / (float(want) + 1e-6), rtol=3 * 2.0 ** -24, atol=0)
 
 
+@pytest.mark.parametrize("sharded", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_buckets_recover_from_a_step_that_is_not_finite(bad, sharded):
+    # Sizes that leave room up to the next 16 bytes behind every tensor, and gradients that are written through their views only.
+    shapes = [(5,), (7,), (0,), (8,), (3, 3)]
+    buckets = ar.GradientBuckets(shapes, device="cpu", shardable=True)
+    params = [torch.nn.Parameter(torch.zeros(s)) for s in shapes]
+    buckets.attach(params)
+    ones, spoilt = [torch.ones(s) for s in shapes], [torch.ones(s) for s in shapes]
+    spoilt[0][2] = bad
+    for write in (buckets.load, lambda gs: [p.grad.add_(g) for p, g in zip(params, gs)]):
+        write(spoilt)
+        assert not math.isfinite(buckets.clip_grad_norm(1.0, sharded=sharded))
+        torch.optim.SGD(params, lr=1.0).zero_grad(set_to_none=False)
+        write(ones)
+        want = torch.tensor(29.0, dtype=torch.float64).sqrt()
+        for same in (False, True):
+            torch.testing.assert_close(buckets.grad_norm(sharded=same).double(), want, rtol=2.0 ** -24, atol=0)
+        buckets.clip_grad_norm(1.0, sharded=sharded)
+        for v in buckets.views:
+            torch.testing.assert_close(v.double(), torch.full_like(v, 1).double() / (want + 1e-6), rtol=3 * 2.0 ** -24, atol=0)
+        torch.optim.SGD(params, lr=1.0).zero_grad(set_to_none=False)
+    assert ar.GradientBuckets([], device="cpu").grad_norm() == 0 and ar.GradientBuckets([(0,)], device="cpu").grad_norm() == 0
+
+
 SHARDED = """
 import math, torch
 import allreduce_proto_b200 as ar
@@ -110,6 +135,36 @@ assert math.isclose(float(sharded), want, rel_tol=1e-6), (float(sharded), want)
 assert math.isclose(float(buckets.grad_norm()), 1.0, rel_tol=1e-5)
 comm.close()
 """
+
+
+AFTER_NAN = """
+import math, torch
+import allreduce_proto_b200 as ar
+comm = ar.Communicator.from_env()
+shapes = [(5,), (7,), (1,), (9,)]   # blocks that begin and end inside of tensors, and between them
+for bucket_bytes in (48, 1 << 20):
+    buckets = ar.GradientBuckets(shapes, device="cpu", comm=comm, shardable=True, symmetric=False, bucket_bytes=bucket_bytes)
+    for first in (math.nan, 1.0, 1.0):
+        buckets.load([torch.full(s, first if i == 0 else 1.0) for i, s in enumerate(shapes)])
+        buckets.reduce_scatter(average=True)
+        norm = float(buckets.grad_norm(sharded=True))
+        assert float(buckets.clip_grad_norm(1.0, sharded=True)) == norm or math.isnan(first)
+        assert math.isnan(norm) if math.isnan(first) else math.isclose(norm, math.sqrt(22), rel_tol=2.0 ** -23), norm
+        buckets.all_gather()
+        for v in buckets.views:
+            want = torch.full_like(v, first / math.sqrt(22))
+            torch.testing.assert_close(v, want, rtol=1e-6, atol=0, equal_nan=True)
+comm.close()
+"""
+
+
+@pytest.mark.parametrize("np_", [2, 3])
+def test_shards_recover_from_a_step_that_is_not_finite(bins, np_, tmp_path):
+    script = tmp_path / "after_nan.py"
+    script.write_text(AFTER_NAN)
+    p = subprocess.run(["timeout", "120s", bins["ibcomm_run"], "-np", str(np_), "-x", f"PYTHONPATH={ROOT}", sys.executable, str(script)],
+                       stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    assert p.returncode == 0, p.stderr[-3000:]
 
 
 @pytest.mark.parametrize("np_", [2, 3])
