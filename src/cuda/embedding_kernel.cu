@@ -1025,12 +1025,19 @@ cudaError_t LaunchEarly(void (*kernel)(Params...), unsigned blocks, int threads,
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
+// Shared memory of the sorts, which depends on the table's rows.  What a kernel is
+// allowed belongs to all threads of the process: it is always what the largest
+// table needs, so that no call takes from another one that is about to launch.
+constexpr size_t ClusterSortBytes(int items, int bits) {
+  return static_cast<size_t>(items) * dev::kClusterThreads * sizeof(uint2) + ((8 + dev::kClusterWarps * 2ull) << bits);
+}
+constexpr size_t SortBytes(int bits) { return (dev::kSortWarps * 4ull) << bits; }
+
 template <int kItems>
 cudaError_t LaunchClusterSort(const dev::SortParams& sort, const SortShape& shape, cudaStream_t stream) {
-  const size_t bins = static_cast<size_t>(1) << shape.bits;
-  const size_t smem = static_cast<size_t>(kItems) * dev::kClusterThreads * sizeof(uint2) + bins * 8 + bins * dev::kClusterWarps * 2;
+  const size_t smem = ClusterSortBytes(kItems, shape.bits);
   auto kernel = dev::ClusterSortKernel<kItems>;
-  cudaError_t e = AllowSharedMemory(kernel, smem);
+  cudaError_t e = AllowSharedMemory(kernel, ClusterSortBytes(kItems, dev::kMostDigitBits));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(shape.blocks));
@@ -1116,8 +1123,8 @@ static cudaError_t LaunchSort(const EmbeddingGradParams& p, dev::SumParams* sum,
     case 2: e = LaunchClusterSort<2>(sort, shape, stream); break;
     case 4: e = LaunchClusterSort<4>(sort, shape, stream); break;
     default: {
-      const size_t smem = (static_cast<size_t>(dev::kSortWarps) << shape.bits) * 4;
-      if (e == cudaSuccess) e = AllowSharedMemory(dev::SortTokensKernel, smem);
+      const size_t smem = SortBytes(shape.bits);
+      e = AllowSharedMemory(dev::SortTokensKernel, SortBytes(dev::kMostDigitBits));
       void* args[] = {&sort};
       if (e == cudaSuccess)
         e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&dev::SortTokensKernel), dim3(static_cast<unsigned>(shape.blocks)), dim3(dev::kSortThreads),

@@ -11,6 +11,7 @@ Tolerances count roundings.  u = 2^-24 is half a step of fp32, `half(t)` half a 
 import math
 import subprocess
 import sys
+import threading
 from pathlib import Path
 
 import pytest
@@ -805,3 +806,29 @@ def test_buckets_recover_from_a_step_that_is_not_a_number(dtype, sharded):
     for v, g in zip(buckets.views, grads):
         w = g.double() * (0.5 / (want.item() + 1e-6))
         within(v, w, (6.5 * U + half(dtype)) * w.abs())
+
+
+@pytest.mark.parametrize("n", [20000, 40000])
+def test_two_threads_with_tables_of_different_sizes(n):
+    # The sorts of both tables are the same kernel (one cluster; cooperative), with digits of 8 and of 10 bits.
+    wants, failures = [], []
+    for rows in (200, 1000):
+        t, g = tokens_of(n, rows, rows), values((n, 8), F32, rows)
+        wants.append((t, g, rows, ar.ops.embedding_grad(t, g, num_rows=rows)))
+    torch.cuda.synchronize()
+
+    def loop(t, g, rows, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(500):
+                    got = ar.ops.embedding_grad(t, g, num_rows=rows)
+                assert torch.equal(got, want)
+        except Exception as e:  # of another thread: pytest does not see it
+            failures.append(repr(e))
+
+    threads = [threading.Thread(target=loop, args=w) for w in wants for _ in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
