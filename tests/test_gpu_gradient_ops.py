@@ -832,3 +832,122 @@ def test_two_threads_with_tables_of_different_sizes(n):
     for thread in threads:
         thread.join()
     assert not failures, failures
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("table", [F32, BF16])
+@pytest.mark.parametrize("n", [200, 30000, 40000])
+def test_gradients_of_every_sort_in_a_graph(n, table, accumulate):
+    # One launch; the sort in a cluster; the cooperative sort: with what is launched early behind them.
+    rows, width = 3001, 40
+    t, g, out = tokens_of(n, rows, 1), values((n, width), BF16, 2), values((rows, width), table, 3)
+    old = out.clone()
+    ar.ops.embedding_grad(t, g, out=out, accumulate=accumulate)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ar.ops.embedding_grad(t, g, out=out, accumulate=accumulate)
+    t.copy_(tokens_of(n, rows, 10))
+    g.copy_(values((n, width), BF16, 20))
+    want = old.clone()
+    ar.ops.embedding_grad(t, g, out=want, accumulate=accumulate)
+    for _ in range(3):
+        out.copy_(old)
+        graph.replay()
+        assert torch.equal(out, want)
+    assert not torch.equal(want, old)
+
+
+class MeanOfTwo:
+    """A communicator whose second rank has no gradients: the mean of a bucket is half of what it holds when the
+    collective runs, on the stream that it is given."""
+    world_size, rank = 2, 0
+
+    def __init__(self):
+        self.calls = []
+
+    def allreduce(self, buf, *, scale, stream, algo, wire):
+        self.calls.append(buf.data_ptr())
+        with torch.cuda.stream(stream):
+            buf.mul_(scale)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_overlapped_mean_sees_the_whole_gradient_of_the_table(tied):
+    # The table's gradient comes some 10 ms late, on a stream of its own.  What is added behind the collective is not halved,
+    # what the collective finds missing is lost to the sum only until then: either is off by half of a gradient.
+    w = torch.nn.Parameter(values((64, 32), F32, 1))
+    head = w if tied else torch.nn.Parameter(values((64, 32), F32, 2))
+    params = [w] if tied else [w, head]
+    t, y = tokens_of(200, 64, 3).clamp(0, 63), values((200, 64), F32, 4)
+    plain = [p.detach().double().requires_grad_(True) for p in params]
+    ((torch.nn.functional.embedding(t, plain[0]) * 2) @ plain[-1].t()).backward(y.double())
+    comm = MeanOfTwo()
+    buckets = ar.GradientBuckets([p.shape for p in params], comm=comm, symmetric=False, bucket_bytes=64 * 32 * 4)
+    buckets.overlap_with_backward(params)
+    side = torch.cuda.Stream()
+    for step in range(1, 4):
+        buckets.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            x = buckets.embedding(0, t, w, scale=2.0)
+        x.register_hook(lambda g: torch.cuda._sleep(20_000_000))
+        torch.cuda.current_stream().wait_stream(side)
+        (x.double() @ head.double().t()).backward(y.double())
+        buckets.finish()
+        assert comm.calls == [b.data_ptr() for b in reversed(buckets.flat)] * step
+        for v, p in zip(buckets.views, plain):
+            # 200 rows at most in a sum, and the roundings of the parts to fp32; halving is exact.
+            within(2 * v.double(), p.grad, 204 * U * (p.grad.abs().max().item() + 200.0))
+    buckets.remove_hooks()
+
+
+GRAPH_BESIDE_GRAPH = """
+import torch
+import allreduce_proto_b200 as ar
+w = torch.randn(50, 16, device="cuda", requires_grad=True)
+t = torch.randint(0, 50, (64,), device="cuda")
+into = torch.zeros(50, 16, device="cuda")
+if ATTACHED:
+    w.grad = into   # as in a bucket
+want = torch.bincount(t, minlength=50)[:, None].expand(50, 16).float()   # of the sum of all rows, exact
+alive = ar.ops.embedding(t, w, **KIND)   # an eager graph of the same leaf, on the default stream
+side = torch.cuda.Stream()
+
+def attempt():
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            ar.ops.embedding(t, w, **KIND).sum().backward()
+    except (RuntimeError, ar.IbcommError) as e:
+        assert "captur" in str(e), e
+        torch.cuda.synchronize()
+        assert w.grad is (into if ATTACHED else None) and not into.any()   # nothing has run
+        return "refused"
+    assert not into.any()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = into if KIND else w.grad
+    assert torch.equal(got, want), got
+    return "right"
+
+first = attempt()
+if first == "refused":
+    alive.sum().backward()   # the eager graph is whole
+    got = into if KIND else w.grad
+    assert torch.equal(got, want), got
+    del got, alive
+    into.zero_()
+    w.grad = into if ATTACHED else None
+    assert attempt() == "right"
+print("done", first)
+"""
+
+
+@pytest.mark.parametrize("kind,attached", [("{}", False), ("{'grad_into': into}", False), ("{'grad_into': into}", True)])
+def test_backward_in_a_graph_is_refused_or_right_beside_an_eager_graph(kind, attached):
+    # Where autograd would make the eager graph's stream wait, CUDA ends the capture; without the eager graph it is captured.
+    child = GRAPH_BESIDE_GRAPH.replace("KIND", kind).replace("ATTACHED", str(attached))
+    p = subprocess.run([sys.executable, "-c", child], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=300)
+    assert p.returncode == 0 and "done" in p.stdout, (p.returncode, p.stdout, p.stderr[-2000:])
