@@ -88,7 +88,7 @@ def grad_norm(tensors: Tensors, *, norm_type: float = 2.0, comm: Optional[Commun
     ``norm_type`` 2 or ``inf`` (the largest magnitude).  CUDA: float32, float64, float16 and bfloat16 in any mixture,
     any dense layout, on the current stream.  ``comm``: the ranks hold different parts (see
     :meth:`GradientBuckets.reduce_scatter`), and the norm is that of all parts; every rank calls.  Without tensors the
-    norm is zero."""
+    norm is zero.  The norm is a number: nothing is differentiated through it."""
     tensors, power = _list(tensors), _power(norm_type)
     if not tensors:
         if _several(comm):

@@ -16,6 +16,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/Event.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -524,6 +525,7 @@ struct EmbeddingBackward : public torch::autograd::Node {
     const at::Tensor& grad = grads[0];
     if (!grad.defined()) return {at::Tensor()};
     TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()), "the embedding's gradient can be taken once, not differentiated again");
+    TORCH_CHECK(!grad._fw_grad(0).defined(), "the embedding's gradient has no forward-mode derivative");
     const at::NoGradGuard no_grad;
     const at::Tensor ids = tokens.unpack(), rows = grad.contiguous();
     try {
@@ -553,6 +555,10 @@ PyObject* Embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!WantArgs(n, 6)) return nullptr;
   int dt, dw;
+  // What is computed from the memory alone would lack the tangent, or be a constant of the trace.
+  if (THPVariable_Check(a[1]) && THPVariable_Unpack(a[1])._fw_grad(0).defined())
+    return Raise(kNotSupported, "the embedding has no forward-mode derivative");
+  if (c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::Tracer)) return Raise(kNotSupported, "the embedding cannot be traced");
   const at::Tensor* tokens = Tensor(a[0], &dt);
   if (tokens == nullptr) return nullptr;
   const at::Tensor* weight = Tensor(a[1], &dw);

@@ -951,3 +951,22 @@ def test_backward_in_a_graph_is_refused_or_right_beside_an_eager_graph(kind, att
     child = GRAPH_BESIDE_GRAPH.replace("KIND", kind).replace("ATTACHED", str(attached))
     p = subprocess.run([sys.executable, "-c", child], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=300)
     assert p.returncode == 0 and "done" in p.stdout, (p.returncode, p.stdout, p.stderr[-2000:])
+
+
+def test_forward_derivatives_are_refused():
+    w = values((20, 8), F32, 1).requires_grad_(True)
+    t = tokens_of(30, 20, 2)
+    forward = torch.autograd.forward_ad
+    y = ar.ops.embedding(t, w)
+    with forward.dual_level():
+        with pytest.raises(ar.IbcommError, match="forward-mode"):
+            ar.ops.embedding(t, forward.make_dual(w.detach(), torch.ones_like(w)))
+        dy = forward.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, w, dy, retain_graph=True)
+    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(g, grad_in_64_bits(t, torch.ones(30, 8, device="cuda"), 20, 1.0)[0].float())
+    # A table that is trained is refused by the tracer itself, which comes first.
+    for table, words in ((w, "requires grad"), (w.detach(), "traced")):
+        with pytest.raises(RuntimeError, match=words):
+            torch.jit.trace(lambda x: ar.ops.embedding(x, table), t)

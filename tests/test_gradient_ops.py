@@ -259,6 +259,20 @@ def test_what_the_call_path_refuses_of_cuda_tensors():
         assert cases[call] in got and got != "nothing", (call, got)
 
 
+def test_derivatives_that_the_embedding_does_not_have_are_refused():
+    # Before anything else is looked at, so on tensors of the host too.
+    w, t = torch.ones(4, 8), torch.zeros(3, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ar.IbcommError, match="forward-mode") as e:
+            ar.ops.embedding(t, torch.autograd.forward_ad.make_dual(w, w))
+        assert e.value.code == ar.NOT_SUPPORTED
+    with pytest.raises(ar.IbcommError, match="traced") as e:
+        torch.jit.trace(lambda x: ar.ops.embedding(x, w), t)
+    assert e.value.code == ar.NOT_SUPPORTED
+    with pytest.raises(ar.IbcommError, match="on the GPU"):  # and nothing is left of either
+        ar.ops.embedding(t, w)
+
+
 def grad_tensors(*items):
     list_ = (_native.GradTensor * len(items))()
     for g, (p, o, n, a, b) in zip(list_, items):
