@@ -33,8 +33,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     ``tokens`` int32 or int64, ``weight`` ``(rows, width)`` float32, float16 or bfloat16; on the current stream.
     Differentiable in ``weight``, backward and once (forward-mode derivatives and ``torch.jit.trace`` are refused): its
     gradient is summed in float32 and comes in the table's type, without the row ``padding_idx``.  With ``grad_into`` (a tensor of the table's shape, such as its view in a gradient bucket) the
-    backward pass adds the gradient there instead, and autograd has nothing to add to ``weight.grad``; lookups that add
-    into one tensor belong on one stream, since nothing orders their backward passes otherwise."""
+    backward pass adds the gradient there instead, and autograd has nothing to add to ``weight.grad``
+    (``torch.autograd.grad`` finds a gradient of zeros, or none); lookups that add into one tensor belong on one stream,
+    since nothing orders their backward passes otherwise.  A table with tensor hooks has its gradient handed to them and
+    added by autograd as usual where ``weight.grad`` is ``grad_into``; elsewhere the backward pass is refused."""
     padding = _check(tokens, padding_idx, weight.shape[0] if weight.dim() == 2 else 0)
     out_code = -1 if out_dtype is None else dtype_code(out_dtype)
     tokens = tokens.contiguous()

@@ -196,8 +196,9 @@ class GradientBuckets:
 
         autograd would zero and fill a tensor of the table's size and add it to the bucket; here only the rows that
         tokens name are read and written.  ``weight`` is the parameter that :meth:`attach` or
-        :meth:`overlap_with_backward` was given in that place; its hook runs as for every other gradient, and the same
-        table may have other uses in the step (a tied output layer; several lookups belong on one stream)."""
+        :meth:`overlap_with_backward` was given in that place; the bucket's hook runs as for every other gradient, and
+        the same table may have other uses in the step (a tied output layer; several lookups belong on one stream).  A
+        table with tensor hooks of its own takes autograd's way, so that they see the gradient.  CUDA tensors only."""
         from ..ops.embedding import embedding
         return embedding(tokens, weight, scale=scale, padding_idx=padding_idx, out_dtype=out_dtype, grad_into=self.views[index])
 

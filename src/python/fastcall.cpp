@@ -520,6 +520,16 @@ struct EmbeddingBackward : public torch::autograd::Node {
   }
   bool released = false;
 
+  bool Hooked() const {
+    const std::shared_ptr<torch::autograd::Node> from = weight.grad_fn();
+    return from != nullptr ? !from->tensor_pre_hooks().empty() : !torch::autograd::impl::hooks(weight).empty();
+  }
+  bool GradIsInto() const {
+    if (!weight.is_leaf() || !weight.grad().defined() || weight.grad().layout() != c10::kStrided) return false;
+    const at::Tensor& grad = weight.grad();
+    return grad.data_ptr() == into.data_ptr() && grad.scalar_type() == into.scalar_type() && grad.is_contiguous();
+  }
+
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     TORCH_CHECK(!released, "the embedding's gradient was taken already; specify retain_graph=True to take it again");
     const at::Tensor& grad = grads[0];
@@ -528,8 +538,11 @@ struct EmbeddingBackward : public torch::autograd::Node {
     TORCH_CHECK(!grad._fw_grad(0).defined(), "the embedding's gradient has no forward-mode derivative");
     const at::NoGradGuard no_grad;
     const at::Tensor ids = tokens.unpack(), rows = grad.contiguous();
+    // A hook of the table is to see, and may change, what is added.
+    const bool hooked = into.defined() && Hooked();
+    TORCH_CHECK(!hooked || GradIsInto(), "the table has a hook, which would not see a gradient that is added to another tensor than weight.grad");
     try {
-      if (!into.defined()) {
+      if (!into.defined() || hooked) {
         at::Tensor out = at::empty(weight.sizes(), weight.options());
         AddGradient(ids, rows, out, padding, scale, false);
         return {out};

@@ -970,3 +970,43 @@ def test_forward_derivatives_are_refused():
     for table, words in ((w, "requires grad"), (w.detach(), "traced")):
         with pytest.raises(RuntimeError, match=words):
             torch.jit.trace(lambda x: ar.ops.embedding(x, table), t)
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_hooks_of_the_table_see_its_gradient(overlap):
+    shapes = [(50, 24), (24,)]
+    buckets = ar.GradientBuckets(shapes)
+    w, b = torch.nn.Parameter(values(shapes[0], F32, 1)), torch.nn.Parameter(values(shapes[1], F32, 2))
+    (buckets.overlap_with_backward if overlap else buckets.attach)([w, b])
+    t, dy = tokens_of(500, 50, 3), values((500, 24), F32, 4)
+    want, bound = grad_in_64_bits(t, dy, 50, 2.0)
+    seen = []
+
+    def step():
+        buckets.zero_()
+        (buckets.embedding(0, t, w, scale=2.0) + b).backward(dy)
+        if overlap:
+            buckets.finish()
+        assert w.grad.data_ptr() == buckets.views[0].data_ptr()
+        return buckets.views[0].clone()
+
+    handle = w.register_hook(lambda g: seen.append(g.clone()) or 4 * g)  # scaling by a power of two is exact
+    got = step()
+    assert len(seen) == 1 and torch.equal(4 * seen[0], got)
+    within(seen[0], want, bound + U * want.abs())
+    handle.remove()
+    within(step(), want, bound + 2 * U * want.abs())
+    assert len(seen) == 1
+    # Added to another tensor, or to that of a table which is no leaf: refused before anything is added.
+    into = torch.zeros(50, 24, device="cuda")
+    w.register_hook(lambda g: seen.append(g))
+    with pytest.raises(RuntimeError, match="hook"):
+        ar.ops.embedding(t, w, grad_into=into).sum().backward()
+    table = w.detach().requires_grad_(True) * 1
+    ar.ops.embedding(t, table, grad_into=into, scale=2.0).backward(dy)
+    within(into, want, bound + 2 * U * want.abs())
+    into.zero_()
+    table.register_hook(lambda g: seen.append(g))
+    with pytest.raises(RuntimeError, match="hook"):
+        ar.ops.embedding(t, table, grad_into=into).sum().backward()
+    assert len(seen) == 1 and not into.any()
