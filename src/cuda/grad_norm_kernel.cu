@@ -202,7 +202,15 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
   const uint32_t thread = threadIdx.x % kNormThreads;
   const TI* in = reinterpret_cast<const TI*>(s.in);
   TO* out = reinterpret_cast<TO*>(s.out);
-  const A c = static_cast<A>(coefficient);
+  // In fp32 a coefficient below the normal numbers (of gradients near the end of the range) would lose its digits: it is
+  // taken 2^126 times as large, and the product is scaled back.
+  const bool tiny = sizeof(A) == 4 && coefficient < 0x1p-126;
+  const A c = static_cast<A>(tiny ? coefficient * 0x1p126 : coefficient);
+  auto scaled = [&](A x) {
+    A v = x * c;
+    if (tiny) v *= static_cast<A>(0x1p-126);
+    return static_cast<AO>(v);
+  };
   const uint64_t base = chunk * kElems;
   constexpr bool kWhole = sizeof(TI) * kN == 32;
   struct Raw {
@@ -218,7 +226,7 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
     VecIO<TI>::Load(r.v[0], a);
     if constexpr (kWhole) VecIO<TI>::Load(r.v[1], a + VecIO<TI>::kN);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) o[e] = static_cast<AO>(a[e] * c);
+    for (int e = 0; e < kN; ++e) o[e] = scaled(a[e]);
     if constexpr (sizeof(TO) * kN == 32) St32(out + i, VecIO<TO>::Store(o), VecIO<TO>::Store(o + VecIO<TO>::kN));
     else St16(out + i, VecIO<TO>::Store(o));
   };
@@ -247,13 +255,13 @@ __device__ __forceinline__ void ScaleChunk(const Span& s, uint32_t chunk, double
       } else {
 #pragma unroll
         for (int e = 0; e < kN; ++e)
-          if (i + e >= s.begin && i + e < s.end) out[i + e] = FromAcc<TO, AO>(static_cast<AO>(ToAcc<A, TI>(in[i + e]) * c));
+          if (i + e >= s.begin && i + e < s.end) out[i + e] = FromAcc<TO, AO>(scaled(ToAcc<A, TI>(in[i + e])));
       }
     }
   } else {
 #pragma unroll 4
     for (uint64_t i = base + thread; i < base + kElems; i += kNormThreads)
-      if (i >= s.begin && i < s.end) out[i] = FromAcc<TO, AO>(static_cast<AO>(ToAcc<A, TI>(in[i]) * c));
+      if (i >= s.begin && i < s.end) out[i] = FromAcc<TO, AO>(scaled(ToAcc<A, TI>(in[i])));
   }
 }
 

@@ -148,7 +148,11 @@ double HostSum(const T* x, size_t n, int power) {
 template <typename T>
 void HostScale(const T* in, T* out, size_t n, double coefficient) {
   const T c = static_cast<T>(coefficient);
-  for (size_t i = 0; i < n; ++i) out[i] = in[i] * c;
+  if (std::isnormal(c) || coefficient == 0.0 || std::isnan(coefficient)) {
+    for (size_t i = 0; i < n; ++i) out[i] = in[i] * c;
+  } else {  // below T's normal numbers, where it would lose its digits
+    for (size_t i = 0; i < n; ++i) out[i] = static_cast<T>(in[i] * coefficient);
+  }
 }
 
 #ifdef USE_CUDA

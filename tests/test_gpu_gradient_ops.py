@@ -1010,3 +1010,24 @@ def test_hooks_of_the_table_see_its_gradient(overlap):
     with pytest.raises(RuntimeError, match="hook"):
         ar.ops.embedding(t, table, grad_into=into).sum().backward()
     assert len(seen) == 1 and not into.any()
+
+
+@pytest.mark.parametrize("bound", [1e-3, 1e-7, 1e-30])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("n", [5, 70001, 40000001])
+@pytest.mark.parametrize("types", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
+def test_clipping_by_coefficients_below_the_normal_numbers(types, n, offset, bound):
+    # The coefficient is 3e-42 or less; what it scales is an ordinary number all the same.
+    a, b = types
+    x = values((n + offset,), a, 1, 1e33)[offset:]
+    x[3] = 3e38
+    out = torch.empty(n + offset, device="cuda", dtype=b)[offset:]
+    norm = norm_of([x], 2)
+    within(ar.ops.clip_grad_norm(x, bound, out=out), norm, norm_rtol(a) * norm.item())
+    want = x.double() * (bound / (norm.item() + 1e-6))
+    assert want[3] > 0.99 * bound
+    # One more rounding to a multiple of fp32's least number where the product is below its normal ones.
+    within(out, want, (6.5 * U + half(b)) * want.abs() + least(F32) + least(b))
+    if a == b:
+        ar.ops.clip_grad_norm(x, bound)
+        assert torch.equal(x, out)

@@ -67,6 +67,18 @@ def test_host_norms_that_are_not_finite():
     assert torch.equal(x, torch.zeros(4))
 
 
+@pytest.mark.parametrize("bound", [1e-3, 1e-7, 1e-30])
+def test_host_clipping_by_coefficients_below_the_normal_numbers(bound):
+    x = torch.tensor([3e38, -1e38, 1e30, 0.0])
+    want = x.double() * (bound / (float(x.double().norm()) + 1e-6))
+    out = torch.empty_like(x)
+    ar.ops.clip_grad_norm(x, bound, out=out)
+    # The product is rounded, to a multiple of the least number where it is below the normal ones.
+    assert torch.all((out.double() - want).abs() <= 3 * 2.0 ** -24 * want.abs() + 2.0 ** -150), (out, want)
+    ar.ops.clip_grad_norm(x, bound)
+    assert torch.equal(x, out)
+
+
 def test_buckets_on_the_host():
     shapes = [(300, 7), (5,), (64, 64)]
     buckets = ar.GradientBuckets(shapes, device="cpu", bucket_bytes=4096, shardable=True)
