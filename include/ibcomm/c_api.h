@@ -141,7 +141,8 @@ int ibcomm_emu_last_status(ibcomm_emu* w, ibcomm_status_report* out);
 /* out[i] = cast(in[i] * scale) on the current device. */
 int ibcomm_copy_scale(const void* in, void* out, size_t len_elements, int dtype_in, int dtype_out, double scale, void* stream);
 
-/* ---- gradients: the norm of a list of tensors, clipping ----
+/* Below, every address is aligned to what it points to.
+ * ---- gradients: the norm of a list of tensors, clipping ----
  * dtypes float32, float64, float16, bfloat16.  power: 2 = root of the sum of squares, 0 = largest magnitude (a NaN
  * anywhere makes either NaN).  `out` = cast(in * min(1, max_norm / (norm + 1e-6))) where clipping: float32 to float32,
  * float16, bfloat16; the 16-bit types to themselves and to float32; float64 to itself.  An `out` is its own `in`

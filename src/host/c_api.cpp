@@ -163,10 +163,14 @@ std::vector<ibcomm::GradTensor> GradTensors(const ibcomm_grad_tensor* tensors, i
 }
 #endif
 
-void CheckSums(const double* sums, int num_sums, const double* work, int norm_dtype) {
+bool Aligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
+void CheckSums(const double* sums, int num_sums, const double* work, const void* norm, int norm_dtype, const double* sum) {
   if (sums != nullptr ? num_sums < 1 : work == nullptr) IBCOMM_FAIL(INVALID_ARGUMENT, "There are neither sums nor a workspace.\n");
   const DType t = CheckDType(norm_dtype);
   if (t != DType::kFloat32 && t != DType::kFloat64) IBCOMM_FAIL(NOT_SUPPORTED, "A norm is float32 or float64.\n");
+  if (!Aligned(sums, 8) || !Aligned(work, 8) || !Aligned(norm, DTypeSize(t)) || !Aligned(sum, 8))
+    IBCOMM_FAIL(INVALID_ARGUMENT, "Sums, the workspace and the norm must be aligned to their type.\n");
 }
 
 void CheckEmbedding(const void* tokens, int tokens_dtype, size_t num_tokens, size_t rows, size_t width, const void* table, int table_dtype, const void* values,
@@ -179,6 +183,8 @@ void CheckEmbedding(const void* tokens, int tokens_dtype, size_t num_tokens, siz
     IBCOMM_FAIL(NOT_SUPPORTED, "Tokens, rows and their width are counted in 31 bits.\n");
   if ((num_tokens > 0 && tokens == nullptr) || (num_tokens > 0 && width > 0 && values == nullptr) || (rows > 0 && width > 0 && table == nullptr))
     IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must have memory.\n");
+  if (!Aligned(tokens, DTypeSize(t)) || !Aligned(table, DTypeSize(CheckDType(table_dtype))) || !Aligned(values, DTypeSize(CheckDType(values_dtype))))
+    IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors must be aligned to their type.\n");
   if (std::isnan(scale)) IBCOMM_FAIL(INVALID_ARGUMENT, "The scale is not a number.\n");
 }
 
@@ -689,7 +695,7 @@ int ibcomm_grad_norm(const ibcomm_grad_tensor* tensors, int count, int power, co
   return Guard([&] {
     NeedCuda();
     CheckGradTensors(tensors, count, power, false, false);
-    CheckSums(sums, num_sums, work, norm_dtype);
+    CheckSums(sums, num_sums, work, norm, norm_dtype, sum);
 #ifdef USE_CUDA
     const std::vector<ibcomm::GradTensor> list = GradTensors(tensors, count);
     const ibcomm::GradNormParams p{list.data(), count, static_cast<ibcomm::GradPower>(power), work, sums, num_sums, norm, norm_dtype == 1, sum, false, 0.0};
@@ -706,7 +712,7 @@ int ibcomm_clip_grads(const ibcomm_grad_tensor* tensors, int count, int power, d
   return Guard([&] {
     NeedCuda();
     CheckGradTensors(tensors, count, power, true, false);
-    CheckSums(sums, num_sums, work, norm_dtype);
+    CheckSums(sums, num_sums, work, norm, norm_dtype, nullptr);
     if (!(max_norm >= 0.0)) IBCOMM_FAIL(INVALID_ARGUMENT, "The largest norm is negative or not a number.\n");
 #ifdef USE_CUDA
     const std::vector<ibcomm::GradTensor> list = GradTensors(tensors, count);

@@ -329,3 +329,20 @@ def test_what_the_c_interface_refuses():
     look = lambda td=3, wd=0, od=0, out=1 << 22: lib.ibcomm_embedding(1 << 20, td, 100, 1 << 21, wd, 50, 64, out, od, 1.0, None)  # noqa: E731
     assert look(td=4) == ar.NOT_SUPPORTED and look(wd=1) == ar.NOT_SUPPORTED and look(od=3) == ar.NOT_SUPPORTED
     assert look(out=None) == ar.INVALID_ARGUMENT and look(out=1 << 21) == ar.INVALID_ARGUMENT
+
+
+def test_what_is_not_aligned_is_refused():
+    # A kernel would fault on it: nothing is launched.
+    lib = _native.lib()
+    one = grad_tensors((4096, 8192, 8, 0, 0))
+    for off in (1, 2, 4):
+        norm = lambda sums=None, work=4096, norm=4096, dt=1, sum_=4096: lib.ibcomm_grad_norm(one, 1, 2, sums, 1, work, norm, dt, sum_, None)  # noqa: E731
+        assert norm(sums=4096 + off) == norm(work=4096 + off) == norm(norm=4096 + off) == norm(sum_=4096 + off) == ar.INVALID_ARGUMENT
+        clip = lambda sums=None, work=4096, norm=4096: lib.ibcomm_clip_grads(one, 1, 2, 1.0, sums, 1, work, norm, 1, None)  # noqa: E731
+        assert clip(sums=4096 + off) == clip(work=4096 + off) == clip(norm=4096 + off) == ar.INVALID_ARGUMENT
+        look = lambda t=0, w=0, o=0: lib.ibcomm_embedding((1 << 20) + t, 3, 100, (1 << 21) + w, 0, 50, 64, (1 << 22) + o, 0, 1.0, None)  # noqa: E731
+        assert look(t=off) == ar.INVALID_ARGUMENT
+        grad = lambda t=0, g=0, o=0: lib.ibcomm_embedding_grad((1 << 20) + t, 3, 9, (1 << 21) + g, 0, (1 << 22) + o, 0, 50, 64, -1, 1.0, 0, None, 0, None)  # noqa: E731
+        assert grad(t=off) == ar.INVALID_ARGUMENT
+        if off < 4:
+            assert look(w=off) == look(o=off) == grad(g=off) == grad(o=off) == ar.INVALID_ARGUMENT
