@@ -103,6 +103,7 @@ void CheckApart(std::vector<Stretch>* all) {
   if (!std::is_sorted(all->begin(), all->end())) std::sort(all->begin(), all->end());
   uintptr_t read = 0, written = 0;  // how far those before reach
   for (const Stretch& s : *all) {
+    if (s.begin == s.end) continue;  // a part without elements shares nothing, wherever it points
     if (s.begin < written || (s.written && s.begin < read))
       IBCOMM_FAIL(INVALID_ARGUMENT, "Tensors that are written must not share memory with another tensor of the call.\n");
     uintptr_t& reach = s.written ? written : read;

@@ -346,3 +346,13 @@ def test_what_is_not_aligned_is_refused():
         assert grad(t=off) == ar.INVALID_ARGUMENT
         if off < 4:
             assert look(w=off) == look(o=off) == grad(g=off) == grad(o=off) == ar.INVALID_ARGUMENT
+
+
+def test_tensors_without_elements_share_no_memory():
+    # Empty parts of the table that is written, or read: nothing to launch, and nothing to refuse.
+    lib = _native.lib()
+    for inside in (1 << 22, (1 << 22) + 64):
+        assert lib.ibcomm_embedding_grad(inside, 3, 0, inside, 0, 1 << 22, 0, 50, 64, -1, 1.0, 1, None, 0, None) == 0
+        assert lib.ibcomm_embedding(inside, 3, 0, 1 << 22, 0, 50, 64, inside, 0, 1.0, None) == 0
+    # One that is not empty.
+    assert lib.ibcomm_embedding_grad(1 << 20, 3, 9, (1 << 22) + 64, 0, 1 << 22, 0, 50, 64, -1, 1.0, 1, None, 0, None) == ar.INVALID_ARGUMENT
