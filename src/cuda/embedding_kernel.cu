@@ -980,6 +980,13 @@ struct SortShape {
   uint32_t per_block;
   int items;  // per thread of a cluster's blocks; 0: the cooperative kernel
 };
+// The list in s->blocks parts for the cooperative kernel, or fewer where that many are not needed.
+void CutSort(uint64_t n, SortShape* s) {
+  uint64_t per = (n + s->blocks - 1) / s->blocks;
+  per = std::max<uint64_t>((per + dev::kSortThreads - 1) / dev::kSortThreads, 1) * dev::kSortThreads;
+  s->per_block = static_cast<uint32_t>(per);
+  s->blocks = static_cast<int>((n + per - 1) / per);
+}
 SortShape ShapeOf(uint64_t n, uint64_t rows) {
   SortShape s;
   int all = 1;  // bits of the keys, 0 .. rows
@@ -997,11 +1004,8 @@ SortShape ShapeOf(uint64_t n, uint64_t rows) {
     return s;
   }
   // A block takes at least 2048 tokens: with fewer the blocks' counts cost more than the tokens.
-  uint64_t blocks = std::min<uint64_t>(std::max<uint64_t>((n + 2047) / 2048, 1), dev::kMostSortBlocks);
-  uint64_t per = (n + blocks - 1) / blocks;
-  per = std::max<uint64_t>((per + dev::kSortThreads - 1) / dev::kSortThreads, 1) * dev::kSortThreads;
-  s.per_block = static_cast<uint32_t>(per);
-  s.blocks = static_cast<int>((n + per - 1) / per);
+  s.blocks = static_cast<int>(std::min<uint64_t>(std::max<uint64_t>((n + 2047) / 2048, 1), dev::kMostSortBlocks));
+  CutSort(n, &s);
   return s;
 }
 
@@ -1093,7 +1097,7 @@ size_t EmbeddingGradWorkBytes(uint64_t n, uint64_t rows, uint64_t width) {
 
 // Sorts the tokens; `sum` gets what lies in the workspace.
 static cudaError_t LaunchSort(const EmbeddingGradParams& p, dev::SumParams* sum, cudaStream_t stream) {
-  const SortShape shape = ShapeOf(p.num_tokens, p.rows);
+  SortShape shape = ShapeOf(p.num_tokens, p.rows);
   char* work = static_cast<char*>(p.work);
   auto take = [&](size_t bytes) {
     char* at = work;
@@ -1125,10 +1129,13 @@ static cudaError_t LaunchSort(const EmbeddingGradParams& p, dev::SumParams* sum,
     default: {
       const size_t smem = SortBytes(shape.bits);
       e = AllowSharedMemory(dev::SortTokensKernel, SortBytes(dev::kMostDigitBits));
-      void* args[] = {&sort};
-      if (e == cudaSuccess)
-        e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(&dev::SortTokensKernel), dim3(static_cast<unsigned>(shape.blocks)), dim3(dev::kSortThreads),
-                                        args, smem, stream);
+      if (e == cudaSuccess) e = LaunchTogether(dev::SortTokensKernel, shape.blocks, dev::kSortThreads, smem, stream, sort);
+      while (e == cudaErrorCooperativeLaunchTooLarge && shape.blocks > 1) {
+        shape.blocks /= 2;
+        CutSort(p.num_tokens, &shape);
+        sort.per_block = shape.per_block;
+        e = LaunchTogether(dev::SortTokensKernel, shape.blocks, dev::kSortThreads, smem, stream, sort);
+      }
       last = (shape.passes - 1) & 1;
     }
   }

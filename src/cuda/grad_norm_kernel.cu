@@ -520,25 +520,6 @@ cudaError_t Launch(void (*kernel)(Params...), int blocks, int threads, int clust
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
-template <typename... Params, typename... Args>
-cudaError_t LaunchTogether(void (*kernel)(Params...), int blocks, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
-  if (smem > 0) {
-    const cudaError_t e = AllowSharedMemory(kernel, smem);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(static_cast<unsigned>(threads));
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeCooperative;
-  attribute.val.cooperative = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 template <int kMost, GradPower P>
 cudaError_t LaunchTyped(const GradNormParams& p, cudaStream_t stream) {
   int full = 0;
@@ -560,12 +541,17 @@ cudaError_t LaunchTyped(const GradNormParams& p, cudaStream_t stream) {
       }
       if (all && p.clip && list.chunks <= kMostHeldChunks) {
         f.num_sums = full / dev::kBlocksPerSm;
-        return LaunchTogether(dev::HeldClipKernel<kMost, P>, f.num_sums, dev::kHeldGroups * dev::kNormThreads, dev::kHeldBytes, stream, list, f,
-                              reinterpret_cast<dev::SumOf<P>*>(p.work));
+        e = AllowSharedMemory(dev::HeldClipKernel<kMost, P>, dev::kHeldBytes);
+        if (e != cudaSuccess) return e;
+        e = LaunchTogether(dev::HeldClipKernel<kMost, P>, f.num_sums, dev::kHeldGroups * dev::kNormThreads, dev::kHeldBytes, stream, list, f,
+                           reinterpret_cast<dev::SumOf<P>*>(p.work));
+        if (e != cudaErrorCooperativeLaunchTooLarge) return e;
       }
       if (all) f.num_sums = static_cast<int>(std::min<uint64_t>(full, (list.chunks + dev::kGroups - 1) / dev::kGroups));
-      if (all && !p.clip && list.chunks <= kMostNormChunks)
-        return LaunchTogether(dev::NormKernel<kMost, P>, f.num_sums, dev::kGroups * dev::kNormThreads, 0, stream, list, reinterpret_cast<dev::SumOf<P>*>(p.work), f);
+      if (all && !p.clip && list.chunks <= kMostNormChunks) {
+        e = LaunchTogether(dev::NormKernel<kMost, P>, f.num_sums, dev::kGroups * dev::kNormThreads, 0, stream, list, reinterpret_cast<dev::SumOf<P>*>(p.work), f);
+        if (e != cudaErrorCooperativeLaunchTooLarge) return e;
+      }
       // The first launch of a call is an ordinary one: what it reads is written by whatever came before.
       e = Launch(dev::GradSumKernel<kMost, P>, f.num_sums, dev::kGroups * dev::kNormThreads, 1, !first, stream, list, reinterpret_cast<dev::SumOf<P>*>(p.work),
                  first ? 1 : 0);

@@ -7,7 +7,32 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "ibcomm/tunables.h"
+
 namespace ibcomm {
+
+// A launch whose blocks wait for one another, refused where they do not fit on the
+// GPU at once: a process may have been given a part of it.  The callers then take
+// kernels that do not wait, or a smaller grid.  IBCOMM_COOPERATIVE_CTAS: the
+// largest such grid, where the runtime does not know of the part.
+template <typename... Params, typename... Args>
+cudaError_t LaunchTogether(void (*kernel)(Params...), int blocks, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+  const int most = Tunable("IBCOMM_COOPERATIVE_CTAS", -1);
+  if (most >= 0 && blocks > 1 && blocks > most) return cudaErrorCooperativeLaunchTooLarge;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeCooperative;
+  attribute.val.cooperative = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+  if (e == cudaErrorCooperativeLaunchTooLarge) cudaGetLastError();  // it is dealt with
+  return e;
+}
 
 // ---- norm of a list of tensors, and clipping (grad_norm_kernel.cu) ----
 // Partial sums that a call may need room for (doubles of its workspace).

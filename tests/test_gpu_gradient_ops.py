@@ -8,6 +8,7 @@ Tolerances count roundings.  u = 2^-24 is half a step of fp32, `half(t)` half a 
 - lookup: the product is rounded to fp32, then to the result's type: u + half(t).
 - gradient: m rows added one by one or in parts, a scale and an addition to the table: at most (m + 2) u of the sum of
   magnitudes, u of the old value, and half a step of the result."""
+import ctypes as C
 import math
 import subprocess
 import sys
@@ -1031,3 +1032,49 @@ def test_clipping_by_coefficients_below_the_normal_numbers(types, n, offset, bou
     if a == b:
         ar.ops.clip_grad_norm(x, bound)
         assert torch.equal(x, out)
+
+
+class KernelNode(C.Structure):
+    _fields_ = [("func", C.c_void_p), ("grid", C.c_uint * 3), ("block", C.c_uint * 3), ("smem", C.c_uint), ("params", C.c_void_p), ("extra", C.c_void_p),
+                ("kernel", C.c_void_p), ("context", C.c_void_p)]
+
+
+def grids_of(call):
+    """(blocks, threads) of the kernels that a call launches."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    driver, raw, count = C.CDLL("libcuda.so.1"), C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(0)
+    assert driver.cuGraphGetNodes(raw, None, C.byref(count)) == 0
+    nodes = (C.c_void_p * count.value)()
+    assert driver.cuGraphGetNodes(raw, nodes, C.byref(count)) == 0
+    found = []
+    for node in nodes:
+        kernel = KernelNode()
+        assert driver.cuGraphKernelNodeGetParams_v2(C.c_void_p(node), C.byref(kernel)) == 0
+        found.append((kernel.grid[0], kernel.block[0]))
+    return found
+
+
+@pytest.mark.parametrize("most", [0, 5, 40])
+def test_where_a_grid_that_waits_does_not_fit(most):
+    # As in a process that has a part of the GPU: kernels that do not wait, or a smaller grid, with the same results.
+    xs = [values((3000001,), F32, 1), values((70001,), BF16, 2)]
+    outs = [torch.empty_like(x) for x in xs]
+    n, rows = 140001, 3001
+    t, g = tokens_of(n, rows, 3), values((n, 24), BF16, 4)
+    calls = [lambda: ar.ops.grad_norm(xs), lambda: ar.ops.clip_grad_norm(xs, 1.0, out=outs), lambda: ar.ops.embedding_grad(t, g, num_rows=rows, dtype=F32)]
+    want, table = norm_of(xs, 2), calls[2]()
+    assert len(grids_of(calls[0])) == len(grids_of(calls[1])) == 1 and max(b for b, threads in grids_of(calls[2]) if threads == 512) > 40
+    ar.utils.set_tunable("IBCOMM_COOPERATIVE_CTAS", most)
+    try:
+        assert len(grids_of(calls[0])) == len(grids_of(calls[1])) == 2
+        assert 1 <= max(b for b, threads in grids_of(calls[2]) if threads == 512) <= max(most, 1)
+        within(calls[0](), want, 5.5 * U * want.item())
+        within(calls[1](), want, 5.5 * U * want.item())
+        for x, o in zip(xs, outs):
+            w = x.double() / (want.item() + 1e-6)
+            within(o, w, (6.5 * U + half(x.dtype)) * w.abs() + least(x.dtype))
+        assert torch.equal(calls[2](), table)
+    finally:
+        ar.utils.set_tunable("IBCOMM_COOPERATIVE_CTAS", -1)
