@@ -520,9 +520,15 @@ struct EmbeddingBackward : public torch::autograd::Node {
   }
   bool released = false;
 
+  // A hook's dictionary stays with the tensor when the hook is taken out of it.
   bool Hooked() const {
     const std::shared_ptr<torch::autograd::Node> from = weight.grad_fn();
-    return from != nullptr ? !from->tensor_pre_hooks().empty() : !torch::autograd::impl::hooks(weight).empty();
+    const auto& hooks = from != nullptr ? from->tensor_pre_hooks() : torch::autograd::impl::hooks(weight);
+    if (hooks.size() != 1) return !hooks.empty();
+    const pybind11::gil_scoped_acquire locked;
+    const auto table = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(weight));
+    const pybind11::object dictionary = pybind11::getattr(table, "_backward_hooks", pybind11::none());
+    return dictionary.is_none() || pybind11::len(dictionary) != 0;
   }
   bool GradIsInto() const {
     if (!weight.is_leaf() || !weight.grad().defined() || weight.grad().layout() != c10::kStrided) return false;

@@ -1078,3 +1078,17 @@ def test_where_a_grid_that_waits_does_not_fit(most):
         assert torch.equal(calls[2](), table)
     finally:
         ar.utils.set_tunable("IBCOMM_COOPERATIVE_CTAS", -1)
+
+
+def test_a_hook_that_was_taken_out_refuses_nothing():
+    t, into = tokens_of(30, 20, 2), torch.zeros(20, 8, device="cuda")
+    want = grad_in_64_bits(t, torch.ones(30, 8, device="cuda"), 20, 1.0)[0].float()  # whole numbers
+    for w in (values((20, 8), F32, 1).requires_grad_(True), values((20, 8), F32, 1).requires_grad_(True) * 1):
+        w.register_hook(lambda g: 2 * g).remove()
+        into.zero_()
+        ar.ops.embedding(t, w, grad_into=into).sum().backward()
+        assert torch.equal(into, want)
+        w.register_hook(lambda g: 2 * g)
+        with pytest.raises(RuntimeError, match="hook"):
+            ar.ops.embedding(t, w, grad_into=into).sum().backward()
+        assert torch.equal(into, want)
