@@ -106,7 +106,9 @@ def clip_grad_norm(tensors: Tensors, max_norm: float, *, out: Optional[Tensors] 
     In place unless ``out`` is given: one tensor per tensor, of the same shape, into which the scaled values go, rounded
     once; float32 may go to the 16-bit types and back (the float32 gradients an optimizer wants of bfloat16 buckets).
     No memory that is written may belong to two tensors of the call.  Gradients whose norm is not finite become NaN, or
-    zero where they were finite and the norm is infinite; check the returned norm to skip such a step."""
+    zero where they were finite and the norm is infinite (NaN with an infinite ``max_norm``); check the returned norm to
+    skip such a step.  What a tensor holds beside gradients, such as the padding of ``GradientBuckets.flat``, becomes NaN
+    with them: hand over the gradients alone, or call :meth:`GradientBuckets.clip_grad_norm`."""
     tensors, power = _list(tensors), _power(norm_type)
     outs = tensors if out is None else _list(out)
     max_norm = float(max_norm)

@@ -173,7 +173,8 @@ int ibcomm_scale_grads_host(const ibcomm_grad_tensor* tensors, int count, double
 int ibcomm_embedding(const void* tokens, int tokens_dtype, size_t num_tokens, const void* weight, int weight_dtype, size_t rows,
                      size_t width, void* out, int out_dtype, double scale, void* stream);
 /* out[v] = cast((accumulate ? out[v] : 0) + scale * sum of grad[t] over the t with tokens[t] == v, v != padding_row), summed in
- * float32 in the order of t.  With accumulate only rows that tokens name are touched, and in float32 tables subnormal numbers
+ * float32 in parts, each in the order of t, that are joined in that order: the parts' lengths depend on the sizes, so the bits
+ * are those of this function only.  With accumulate only rows that tokens name are touched, and in float32 tables subnormal numbers
  * are added as zero.  padding_row -1 = none.  `work`: as many bytes as ibcomm_embedding_grad_work tells, on a boundary of 256
  * bytes; not used by two calls at a time.  No tensor that is written shares memory with another of the call. */
 int ibcomm_embedding_grad_work(size_t num_tokens, size_t rows, size_t width, size_t* bytes);

@@ -205,8 +205,10 @@ __device__ __forceinline__ uint32_t KeyOf(const SortParams& p, uint32_t t) {
 // A least-significant-digit radix sort, cooperative: a block's part of the list
 // is cut into one part per warp, a digit's count of every warp gives the places.
 // A warp places 32 elements at a time in their order, so every pass is stable.
-// Equal digits in a warp are found by one ballot per bit (in the cluster's kernel,
-// 16384 tokens, 14.1 us against 16.2 with `match.any`).  131072 tokens of 32000 rows: 24 us, two digits of 8 bits.
+// Equal digits in a warp are found by one ballot per bit (in the cluster's kernel
+// as it was then, 16384 tokens, 14.1 us against 16.2 with `match.any`).  131072
+// tokens of 32000 rows, two digits of 8 bits: 24 us by itself with cold caches, 22
+// among the kernels of a call, where the next one is set up beside it.
 __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
   extern __shared__ uint32_t warp_counts[];  // kSortWarps x bins
   LetNextStart();
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kSortThreads) SortTokensKernel(SortParams p) {
 // memory: a thread holds kItems elements in registers, counts go from block to
 // block through distributed shared memory, elements are placed in the shared
 // memory of the block that has them in the next pass.  Against the cooperative
-// kernel, tokens of 50000 rows: 2048 8.5 us against 18.5, 16384 13.5 against 22,
+// kernel, tokens of 50000 rows, by itself: 2048 8.5 us against 18.5, 16384 13 against 22,
 // 32768 20.3 against 22.2, 65536 35 against 23 (there are only eight SMs to place
 // the elements), so lists of up to 32768 are taken.
 constexpr int kClusterThreads = 1024;
