@@ -32,11 +32,12 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
 
     ``tokens`` int32 or int64, ``weight`` ``(rows, width)`` float32, float16 or bfloat16; on the current stream.
     Differentiable in ``weight``, backward and once (forward-mode derivatives and ``torch.jit.trace`` are refused): its
-    gradient is summed in float32 and comes in the table's type, without the row ``padding_idx``.  With ``grad_into`` (a tensor of the table's shape, such as its view in a gradient bucket) the
-    backward pass adds the gradient there instead, and autograd has nothing to add to ``weight.grad``
-    (``torch.autograd.grad`` finds a gradient of zeros, or none); lookups that add into one tensor belong on one stream,
-    since nothing orders their backward passes otherwise.  A table with tensor hooks has its gradient handed to them and
-    added by autograd as usual where ``weight.grad`` is ``grad_into``; elsewhere the backward pass is refused."""
+    gradient is summed in float32 and comes in the table's type, without the row ``padding_idx``.  With ``grad_into`` (a
+    tensor of the table's shape, such as its view in a gradient bucket) the backward pass adds the gradient there instead,
+    and autograd has nothing to add to ``weight.grad`` (``torch.autograd.grad`` finds a gradient of zeros, or none); lookups
+    that add into one tensor belong on one stream, since nothing orders their backward passes otherwise.  A table with
+    tensor hooks has its gradient handed to them and added by autograd as usual where ``weight.grad`` is ``grad_into``;
+    elsewhere the backward pass is refused."""
     padding = _check(tokens, padding_idx, weight.shape[0] if weight.dim() == 2 else 0)
     out_code = -1 if out_dtype is None else dtype_code(out_dtype)
     tokens = tokens.contiguous()
@@ -58,8 +59,8 @@ def embedding_grad(tokens: torch.Tensor, grad: torch.Tensor, *, out: Optional[to
     are added to it and only rows that tokens name are touched (in float32 tables subnormal numbers, below 1.2e-38, are
     added as zero).  Without ``out`` a table of ``num_rows`` rows in ``dtype``
     (default: ``grad``'s) is made.  Types float32, float16, bfloat16 in any mixture; sums in float32, rounded once.  Not
-    differentiable itself.  ``tokens`` and ``grad`` may come from several ranks (``all_gather`` both): with many rows that few tokens name, that is
-    less to send than the table's gradient."""
+    differentiable itself.  ``tokens`` and ``grad`` may come from several ranks (``all_gather`` both): with many rows that
+    few tokens name, that is less to send than the table's gradient."""
     if out is None:
         if num_rows is None or num_rows < 0 or accumulate:
             raise IbcommError(_native.INVALID_ARGUMENT, "give out, or num_rows without accumulate")
