@@ -64,7 +64,8 @@ class GradientBuckets:
         self.plan = plan_buckets(numels, esize, bucket_bytes)
         self.flat: list[torch.Tensor] = []
         self.views: list[torch.Tensor] = [None] * len(self.shapes)  # type: ignore[list-item]
-        # What a bucket holds of gradients, without the places in between and behind: tensors that follow one another make one run.
+        # What a bucket holds of gradients, without the places in between and behind: tensors that follow one
+        # another make one run.
         self._runs: list[torch.Tensor] = []
         self._own_runs: list[torch.Tensor] = []  # inside this rank's blocks
         for idxs in self.plan:
